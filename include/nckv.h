@@ -332,6 +332,13 @@ NCKV_API int nckv_append_rope_norm_paged(const void *q_in, const void *k_in, con
                                 const void *cos, const void *sin, int B, int T_new, int Hq, int Hkv, int D,
                                 int page_tokens, int max_pages, int n_pages, int64_t page_stride, int64_t token_stride,
                                 int rope_len, float qk_scale, float eps, int32_t *status, void *stream);
+/* With new_tokens (int32 per row, or NULL: T_new for all) only the first new_tokens[b] of a row's T_new slots hold a token; the others
+ * write nothing to the pools and zeros to q_out. */
+NCKV_API int nckv_append_rope_norm_paged_counts(const void *q_in, const void *k_in, const void *v_in, void *q_out, void *k_pool,
+                                void *v_pool, const int32_t *block_table, const int32_t *cache_seqlens, const int32_t *new_tokens,
+                                const void *cos, const void *sin, int B, int T_new, int Hq, int Hkv, int D,
+                                int page_tokens, int max_pages, int n_pages, int64_t page_stride, int64_t token_stride,
+                                int rope_len, float qk_scale, float eps, int32_t *status, void *stream);
 NCKV_API int nckv_decode_attn_paged(const void *q, const void *k_pool, const void *v_pool, const int32_t *block_table,
                            const int32_t *cache_seqlens, void *out, float *out_f32, float *lse_out, int B, int Hq,
                            int Hkv, int D, int page_tokens, int max_pages, int n_pages, int64_t page_stride,
@@ -339,6 +346,19 @@ NCKV_API int nckv_decode_attn_paged(const void *q, const void *k_pool, const voi
                            size_t workspace_bytes, void *stream);
 NCKV_API int nckv_paged_fill(const void *src_k, const void *src_v, void *k_pool, void *v_pool, const int32_t *jobs,
                     int n_jobs, int L, int Hkv, int D, int T_src, int page_tokens, int n_pages, void *stream);
+
+/*
+ * Attention of a chunk of T new tokens per row over pages that hold them already (nckv_append_rope_norm_paged_counts ahead of it).  Row b has
+ * cache_seqlens[b] keys before the chunk and new_tokens[b] tokens in it (new_tokens NULL: T); query t < new_tokens[b] of q (B, T, Hq, D) sees the
+ * keys of positions [max(0, p - window_left), p], p = cache_seqlens[b] + t (window_left < 0: from 0).  out (B, T, Hq, D) is zero in slots without
+ * a token and in rows that don't fit their table (flagged).  Hq / Hkv at most 128.  The workspace (256-byte aligned, at least
+ * nckv_prefill_attn_paged_workspace_bytes, which is 0 where none is needed or the sizes are refused) is the call's own.
+ */
+NCKV_API size_t nckv_prefill_attn_paged_workspace_bytes(int B, int T, int Hq, int Hkv, int page_tokens, int max_pages, int window_left);
+NCKV_API int nckv_prefill_attn_paged(const void *q, const void *k_pool, const void *v_pool, const int32_t *block_table,
+                                const int32_t *cache_seqlens, const int32_t *new_tokens, void *out, int B, int T, int Hq, int Hkv,
+                                int D, int page_tokens, int max_pages, int n_pages, int64_t page_stride, int64_t token_stride,
+                                int window_left, void *workspace, size_t workspace_bytes, int32_t *status, void *stream);
 
 /*
  * nckv_append_rope_norm and nckv_decode_attn (or their paged forms: block_table given, T_max the tokens of a page, batch_stride the

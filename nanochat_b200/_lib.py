@@ -54,6 +54,10 @@ SIGNATURES = {
     "nckv_paged_tile_tokens": (c_int, []),
     "nckv_append_rope_norm_paged": (c_int, [c_void_p] * 10 + [c_int] * 8 + [c_i64, c_i64, c_int, c_float, c_float,
                                                              c_void_p, c_void_p]),
+    "nckv_append_rope_norm_paged_counts": (c_int, [c_void_p] * 11 + [c_int] * 8 + [c_i64, c_i64, c_int, c_float, c_float,
+                                                                    c_void_p, c_void_p]),
+    "nckv_prefill_attn_paged_workspace_bytes": (c_size_t, [c_int] * 7),
+    "nckv_prefill_attn_paged": (c_int, [c_void_p] * 7 + [c_int] * 8 + [c_i64, c_i64, c_int, c_void_p, c_size_t, c_void_p, c_void_p]),
     "nckv_decode_attn_paged": (c_int, [c_void_p] * 8 + [c_int] * 7 + [c_i64, c_i64, c_int, c_int, c_void_p, c_size_t,
                                                         c_void_p]),
     "nckv_paged_fill": (c_int, [c_void_p] * 5 + [c_int] * 7 + [c_void_p]),

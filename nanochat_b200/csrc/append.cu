@@ -36,6 +36,7 @@ struct AppendParams {
     // T_max is then max_pages * page_tokens and cache_batch_stride the distance between pages
     const int32_t *block_table;
     int page_tokens, max_pages, n_pages;
+    const int32_t *new_tokens;  // optional, per row: how many of its T_new slots hold a token; q_out is zero in the others
     // distance between the tokens of q_in / k_in / v_in in 16-byte units (heads of a token are packed); lets the
     // three be column slices of one projection output
     long long q_stride, k_stride, v_stride;
@@ -76,6 +77,12 @@ __global__ void __launch_bounds__(256) append_rope_norm_kernel(const AppendParam
         hi[i] = reinterpret_cast<const uint2 *>(row)[16 + j];
     }
     const int len = p.cache_seqlens[b];          // sequence position of token 0 (drives RoPE)
+    int n_new = p.T_new;
+    if (p.new_tokens) {
+        const int n = p.new_tokens[b];
+        n_new = min(max(n, 0), p.T_new);
+        if (n != n_new && live && j == 0 && first == 0 && t == 0) atomicOr(p.status, (int)(n < 0 ? NCKV_ST_BAD_SEQLEN : NCKV_ST_OVERFLOW));
+    }
     int wslot = p.write_slots ? p.write_slots[b] : len;  // cache index of token 0
     if (p.split.block > 0 && len >= 0)
         wslot = (len / p.split.block) % p.split.world == p.split.rank
@@ -84,10 +91,12 @@ __global__ void __launch_bounds__(256) append_rope_norm_kernel(const AppendParam
     if (len < 0 || wslot < -1) {
         if (live && j == 0 && first == 0 && t == 0) atomicOr(p.status, (int)NCKV_ST_BAD_SEQLEN);
         ok = false;
-    } else if ((wslot >= 0 && wslot + p.T_new > p.T_max) || (p.rope_len > 0 && len + p.T_new > p.rope_len)) {
+    } else if ((wslot >= 0 && wslot + n_new > p.T_max) || (p.rope_len > 0 && len + n_new > p.rope_len)) {
         if (live && j == 0 && first == 0 && t == 0) atomicOr(p.status, (int)NCKV_ST_OVERFLOW);
         ok = false;
     }
+    const bool empty = ok && t >= n_new;  // a slot without a token
+    ok = ok && !empty;
     const bool write_kv = ok && wslot >= 0;  // -1: this row's token belongs to another shard
     uint2 c = make_uint2(0, 0), s = make_uint2(0, 0);
     if (ok && p.rope_len > 0) {
@@ -125,7 +134,8 @@ __global__ void __launch_bounds__(256) append_rope_norm_kernel(const AppendParam
                 hi[i] = d;
             }
         }
-        if (slot >= heads_per_tok || !ok || (kind != 0 && !in_cache)) continue;
+        if (empty && kind == 0) lo[i] = hi[i] = make_uint2(0, 0);
+        if (slot >= heads_per_tok || !(ok || (empty && kind == 0)) || (kind != 0 && !in_cache)) continue;
         uint2 *dst = kind == 0 ? reinterpret_cast<uint2 *>(p.q_out + ((long long)tok * p.Hq + h) * 16)
                                : reinterpret_cast<uint2 *>((kind == 1 ? p.k_cache : p.v_cache) + dst_off + (long long)h * NCKV_D);
         dst[j] = lo[i];
@@ -205,7 +215,7 @@ static int append_rope_norm_impl(const void *q_in, const void *k_in, const void 
                                  int64_t cache_token_stride, int rope_len, float qk_scale, float eps,
                                  int32_t *status, void *stream, const int32_t *block_table = nullptr,
                                  int page_tokens = 0, int max_pages = 0, int n_pages = 0, int64_t q_token_stride = 0,
-                                 int64_t k_token_stride = 0, int64_t v_token_stride = 0) {
+                                 int64_t k_token_stride = 0, int64_t v_token_stride = 0, const int32_t *new_tokens = nullptr) {
     using namespace nckv;
     if ((q_token_stride && (q_token_stride % 8 || q_token_stride < (int64_t)Hq * D)) ||
         (k_token_stride && (k_token_stride % 8 || k_token_stride < (int64_t)Hkv * D)) ||
@@ -249,6 +259,7 @@ static int append_rope_norm_impl(const void *q_in, const void *k_in, const void 
     p.split = split;
     p.block_table = block_table;
     p.page_tokens = page_tokens; p.max_pages = max_pages; p.n_pages = n_pages;
+    p.new_tokens = new_tokens;
     p.q_stride = q_token_stride ? q_token_stride / 8 : (long long)Hq * 16;
     p.k_stride = k_token_stride ? k_token_stride / 8 : (long long)Hkv * 16;
     p.v_stride = v_token_stride ? v_token_stride / 8 : (long long)Hkv * 16;
@@ -312,11 +323,11 @@ int nckv_append_rope_norm_split(const void *q_in, const void *k_in, const void *
                                  cache_batch_stride, cache_token_stride, rope_len, qk_scale, eps, status, stream);
 }
 
-int nckv_append_rope_norm_paged(const void *q_in, const void *k_in, const void *v_in, void *q_out, void *k_pool,
-                                void *v_pool, const int32_t *block_table, const int32_t *cache_seqlens,
-                                const void *cos, const void *sin, int B, int T_new, int Hq, int Hkv, int D,
-                                int page_tokens, int max_pages, int n_pages, int64_t page_stride, int64_t token_stride,
-                                int rope_len, float qk_scale, float eps, int32_t *status, void *stream) {
+int nckv_append_rope_norm_paged_counts(const void *q_in, const void *k_in, const void *v_in, void *q_out, void *k_pool,
+                                       void *v_pool, const int32_t *block_table, const int32_t *cache_seqlens,
+                                       const int32_t *new_tokens, const void *cos, const void *sin, int B, int T_new, int Hq, int Hkv, int D,
+                                       int page_tokens, int max_pages, int n_pages, int64_t page_stride, int64_t token_stride,
+                                       int rope_len, float qk_scale, float eps, int32_t *status, void *stream) {
     if (!block_table || page_tokens <= 0 || max_pages <= 0 || n_pages <= 0 ||
         (long long)page_tokens * max_pages > 0x3fffffffLL) {
         nckv::set_error("append_rope_norm_paged: bad paging (page_tokens=%d max_pages=%d n_pages=%d)", page_tokens,
@@ -325,7 +336,17 @@ int nckv_append_rope_norm_paged(const void *q_in, const void *k_in, const void *
     }
     return append_rope_norm_impl(q_in, k_in, v_in, q_out, k_pool, v_pool, cache_seqlens, nullptr, nckv::KvSplit{0, 0, 0},
                                  cos, sin, B, T_new, Hq, Hkv, D, page_tokens * max_pages, page_stride, token_stride,
-                                 rope_len, qk_scale, eps, status, stream, block_table, page_tokens, max_pages, n_pages);
+                                 rope_len, qk_scale, eps, status, stream, block_table, page_tokens, max_pages, n_pages, 0, 0, 0, new_tokens);
+}
+
+int nckv_append_rope_norm_paged(const void *q_in, const void *k_in, const void *v_in, void *q_out, void *k_pool,
+                                void *v_pool, const int32_t *block_table, const int32_t *cache_seqlens,
+                                const void *cos, const void *sin, int B, int T_new, int Hq, int Hkv, int D,
+                                int page_tokens, int max_pages, int n_pages, int64_t page_stride, int64_t token_stride,
+                                int rope_len, float qk_scale, float eps, int32_t *status, void *stream) {
+    return nckv_append_rope_norm_paged_counts(q_in, k_in, v_in, q_out, k_pool, v_pool, block_table, cache_seqlens, nullptr, cos, sin, B, T_new,
+                                              Hq, Hkv, D, page_tokens, max_pages, n_pages, page_stride, token_stride, rope_len, qk_scale, eps,
+                                              status, stream);
 }
 
 int nckv_append(const void *k_in, const void *v_in, void *k_cache, void *v_cache,
@@ -357,6 +378,7 @@ int nckv_append(const void *k_in, const void *v_in, void *k_cache, void *v_cache
     p.split = KvSplit{0, 0, 0};
     p.block_table = nullptr;
     p.page_tokens = p.max_pages = p.n_pages = 0;
+    p.new_tokens = nullptr;
     p.q_stride = 0;
     p.k_stride = p.v_stride = (long long)Hkv * 16;
     return launch_append(p, static_cast<cudaStream_t>(stream));

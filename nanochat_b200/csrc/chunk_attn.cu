@@ -1,0 +1,1006 @@
+// Attention of a chunk of new tokens per row over a paged cache that holds them already (speculative tokens, portions of
+// prompts, whole prompts), on the 5th-generation tensor cores.
+//
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^((q . k_j) scale log2(e) - m),   j in [max(0, L + t - window), L + t]
+//
+// for query t < n of a row with L keys before its n new ones.  Running maximum and sum in fp32, one pass over the keys; P is
+// rounded to bf16 (2^-9 of a term of the sum, the type of V) because the tensor core takes it beside V in that type.
+//
+// A tile is CH_M = 128 query rows of one (row, kv head): the G query heads of the group at 128 / G consecutive tokens, row = token * G +
+// head, so keys and values are read once for the whole group.  It walks over its keys in tiles of 64, cut at multiples of 64.  Pages
+// hold a multiple of 48 tokens: a tile is copied in boxes of gcd(64, page) keys, each of which lies in one page.
+// The pipeline is that of the dense kernel (prefill_attn.cu): two persistent CTAs per SM, a copying thread, a thread that issues S = Q K^T two
+// tiles ahead and O += P V, and one softmax thread per query row that takes its scores out of tensor memory and puts P back over them.
+//
+// What a CTA works through, found by every role from the rows' lengths alone:
+//   stretches: the sequence of all key tiles of all tiles of queries, (row, kv head) by (row, kv head), is cut into equal stretches, one per
+//     CTA; tiles of queries that lie in several leave partial sums.  Balanced to a key tile whatever the lengths.  Where tiles of queries share
+//     keys (more than one per row) and the keys are more than L2 holds, up to CH_PHASES groups of pairs are cut one after the other.
+//   a deal: tiles of queries of rows of like lengths, enough of them to fill the CTAs' rounds, go to the CTAs uncut, longest first, back and
+//     forth, as in the dense kernel.
+// chunk_finish_kernel adds up partial sums in the order of the keys: results don't depend on timing.
+//
+// Every barrier wait is bounded; one that runs out sets NCKV_ST_TIMEOUT, the CTA stops issuing work, waits for its copies, frees its
+// tensor memory and returns.
+#include <math.h>
+
+#include "nckv_common.cuh"
+#include "tc05.cuh"
+
+namespace nckv {
+
+constexpr int CH_M = 128, CH_N = 64;
+constexpr int CH_STAGES = 2, CH_VSTAGES = 3;  // of K and of V
+constexpr int CH_THREADS = CH_M + 64;         // softmax threads, the issuing warp, the copying warp
+constexpr int CH_Q_BYTES = CH_M * NCKV_D * 2, CH_KV_BYTES = CH_N * NCKV_D * 2;
+constexpr int CH_TMEM_COLS = 256;  // S / P buffers [0, 64), [64, 128); O [128, 256)
+constexpr int CH_PHASES = 4;       // most groups of pairs that are cut one after the other
+constexpr int CH_MIN_TILES = 1;    // shortest stretch of a CTA
+constexpr int CH_PLAN = 16;        // words of the plan ahead of the tiles' places: begin and stretch of every phase, and its number of stretches
+constexpr long long CH_PART_BYTES = 160LL << 20, CH_PHASE_BYTES = 48LL << 20;
+
+struct ChunkParams {
+    const int32_t *table, *seqlens, *new_tokens;  // new_tokens may be null: T for every row
+    const __nv_bfloat16 *v_pool;
+    __nv_bfloat16 *out;
+    int32_t *plan;   // [2 f], [2 f + 1]: first key tile and stretch of phase f (0: dealt); from CH_PLAN on, for every row: key tiles before it,
+                     // key tiles per kv head, then key tiles before each of its tiles of queries
+    float *part_ml;  // (slots, part_rows, 2): maximum and sum
+    float *part_o;   // (slots, part_rows, 128), not divided by the sum
+    int32_t *status;
+    int B, T, Hq, Hkv, G, tile_tokens, n_qtiles;
+    int page_tokens, max_pages, n_pages, capacity, box;
+    int64_t page_stride, token_stride;
+    int window_left;
+    int phases, part_rows;        // phases 0: nothing is cut
+    int phase_pairs;              // (row, kv head) pairs of a phase
+    int group_pairs, n_groups;    // of a deal
+    float scale_log2;
+};
+
+// A row's lengths; n = 0 for one that can't be (its outputs are zeros).
+struct ChunkRow {
+    int L, n;
+};
+__device__ __forceinline__ ChunkRow chunk_row(const ChunkParams &p, int b) {
+    ChunkRow r;
+    r.L = __ldg(p.seqlens + b);
+    r.n = p.new_tokens ? min(max(__ldg(p.new_tokens + b), 0), p.T) : p.T;
+    if (r.L < 0 || (long long)r.L + r.n > p.capacity) r.L = r.n = 0;
+    return r;
+}
+
+// Key tiles [first, first + count) that any of the tokens [t0, t0 + tile_tokens) of a row sees.
+struct ChunkSpan {
+    int kv_lo, kv_hi, first, count;
+};
+__device__ __forceinline__ ChunkSpan chunk_span(const ChunkParams &p, const ChunkRow &r, int t0) {
+    ChunkSpan s;
+    s.kv_lo = p.window_left >= 0 ? max(0, r.L + t0 - p.window_left) : 0;
+    s.kv_hi = r.L + min(t0 + p.tile_tokens, r.n);
+    s.first = s.kv_lo / CH_N;
+    s.count = t0 < r.n ? (s.kv_hi + CH_N - 1) / CH_N - s.first : 0;
+    return s;
+}
+
+// A CTA's piece of work: key tiles [tile0, tile0 + n_tiles) of one tile of queries.
+struct ChunkUnit {
+    int b, hkv, t0, L, n;
+    int kv_lo, kv_hi, tile0, n_tiles;
+    int slot;  // where the partial sums go; -1: all keys, the output is written
+};
+
+// Where a CTA's stretch of a phase lies: [at, end) in the sequence of key tiles, beginning at key tile `off` of a tile of queries.
+struct ChunkStretch {
+    int at, end, b, hkv, qt, off;
+};
+
+// Walks over a CTA's pieces of work.
+struct ChunkCursor {
+    ChunkUnit u;
+    int t;    // key tile inside the piece
+    int seq;  // number of the piece among the CTA's
+    bool valid;
+    int phase;  // -1: dealt
+    int at;     // next key tile of the stretch, or next round of the deal
+    int begin, end, qt, off;
+    ChunkSpan span;
+
+    __device__ __forceinline__ void item(const ChunkParams &p) {
+        u.t0 = qt * p.tile_tokens;
+        span = chunk_span(p, ChunkRow{u.L, u.n}, u.t0);
+    }
+    __device__ __forceinline__ void row(const ChunkParams &p, int b) {
+        const ChunkRow r = chunk_row(p, b);
+        u.b = b;
+        u.L = r.L;
+        u.n = r.n;
+    }
+    __device__ __forceinline__ bool enter(const ChunkParams &p, const ChunkStretch *stretches) {  // the next phase with something in it
+        for (; phase < p.phases; ++phase) {
+            const ChunkStretch s = stretches[phase];
+            if (s.at >= s.end) continue;
+            at = begin = s.at;
+            end = s.end;
+            row(p, s.b);
+            u.hkv = s.hkv;
+            qt = s.qt;
+            off = s.off;
+            item(p);
+            return true;
+        }
+        return false;
+    }
+    __device__ __forceinline__ void start(const ChunkParams &p, const ChunkStretch *stretches, bool dealt) {
+        seq = -1;
+        valid = true;
+        at = end = begin = 0;
+        phase = dealt ? -1 : 0;
+        if (!dealt) valid = enter(p, stretches);
+        if (valid) load(p, stretches);
+    }
+    __device__ __forceinline__ void load(const ChunkParams &p, const ChunkStretch *stretches) {
+        t = 0;
+        ++seq;
+        const int grid = (int)gridDim.x, c = (int)blockIdx.x;
+        if (phase >= 0) {
+            if (at >= end) {
+                ++phase;
+                valid = enter(p, stretches);
+                if (!valid) return;
+            } else {
+                while (off >= span.count) {  // ends: there are tiles behind `at`
+                    off = 0;
+                    if ((++qt) * p.tile_tokens >= u.n) {
+                        qt = 0;
+                        if (++u.hkv == p.Hkv) {
+                            u.hkv = 0;
+                            do row(p, u.b + 1);
+                            while (u.n == 0);
+                        }
+                    }
+                    item(p);
+                }
+            }
+            u.kv_lo = span.kv_lo;
+            u.kv_hi = span.kv_hi;
+            u.n_tiles = min(span.count - off, end - at);
+            u.tile0 = span.first + off;
+            u.slot = u.n_tiles == span.count ? -1 : (phase * grid + c) * 2 + (at != begin);
+            off += u.n_tiles;
+            at += u.n_tiles;
+            return;
+        }
+        const int pairs = p.B * p.Hkv, per_group = p.group_pairs * p.n_qtiles;
+        for (;; ++at) {
+            const long long idx = (long long)at * grid + ((at & 1) ? grid - 1 - c : c);  // dealt back and forth
+            if (idx >= (long long)pairs * p.n_qtiles) {  // none in this round, then none later
+                valid = false;
+                return;
+            }
+            const int grp = min((int)idx / per_group, p.n_groups - 1), in_grp = (int)idx - grp * per_group;
+            const int grp_pairs = grp == p.n_groups - 1 ? pairs - grp * p.group_pairs : p.group_pairs;
+            const int pair = grp * p.group_pairs + in_grp % grp_pairs;
+            qt = p.n_qtiles - 1 - in_grp / grp_pairs;  // all pairs' longest tiles first
+            row(p, pair / p.Hkv);
+            if (qt * p.tile_tokens >= u.n) continue;
+            u.hkv = pair - u.b * p.Hkv;
+            item(p);
+            u.kv_lo = span.kv_lo;
+            u.kv_hi = span.kv_hi;
+            u.n_tiles = span.count;
+            u.tile0 = span.first;
+            u.slot = -1;
+            ++at;
+            return;
+        }
+    }
+    __device__ __forceinline__ void advance(const ChunkParams &p, const ChunkStretch *stretches) {
+        if (++t >= u.n_tiles) load(p, stretches);
+    }
+    __device__ __forceinline__ bool last_of_unit() const { return t == u.n_tiles - 1; }
+};
+
+// Whether uncut tiles dealt to the CTAs take less than stretches: rows' key tiles per kv head between `least` and `most`, `items` tiles of
+// queries of `tiles` key tiles altogether.  A partial sum of 128 rows (64 KB written and read) costs some 3 tiles, a piece 2.
+__device__ __forceinline__ bool chunk_dealt(const ChunkParams &p, int least, int most, long long tiles, int items, int longest, int grid) {
+    if (p.phases == 0) return true;
+    if (p.n_qtiles == 1 || items < grid || most - least > most / 8) return false;
+    const float each = (float)tiles / items, per_cta = (float)tiles / grid, rounds = (float)items / grid;
+    const bool alike = longest < 1.5f * each;  // then rounds are whole, else the short tiles fill them up
+    const float deal = alike ? ceilf(rounds) * (each + 2.f) : fmaxf(per_cta * 1.05f, (float)longest) + 2.f * rounds;
+    return deal <= per_cta + 2.f * rounds + 7.f * p.phases;
+}
+
+__device__ __forceinline__ bool not_finite2(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
+
+// What values that are not finite add to a query row: they were taken out of the shared tiles that some rows don't see all of (zero
+// times infinity would reach those rows).  Rare, so it reads the pages again.
+__device__ __noinline__ float chunk_not_finite(const ChunkParams &p, const ChunkUnit u, int pos, int channel) {
+    float sum = 0.f;
+    const int hi = min(pos + 1, u.kv_hi), lo = p.window_left >= 0 ? max(pos - p.window_left, 0) : 0;
+    const int first_pos = u.L + u.t0, last_pos = u.L + min(u.t0 + p.tile_tokens, u.n) - 1;
+    for (int t = 0; t < u.n_tiles; ++t) {
+        const int key0 = (u.tile0 + t) * CH_N;
+        if (!(key0 + CH_N - 1 > first_pos || (p.window_left >= 0 && key0 < last_pos - p.window_left))) continue;
+        for (int j = max(lo, key0); j < min(hi, key0 + CH_N); ++j) {
+            const int idx = j / p.page_tokens, page = p.table[(long long)u.b * p.max_pages + idx];
+            if (page < 0 || page >= p.n_pages) continue;
+            const float v = __bfloat162float(p.v_pool[page * p.page_stride + (long long)(j - idx * p.page_tokens) * p.token_stride + u.hkv * NCKV_D + channel]);
+            if (!(fabsf(v) <= 3.4e38f)) sum += v;
+        }
+    }
+    return sum;
+}
+
+__global__ void __launch_bounds__(CH_THREADS, 2)
+chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                  const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ ChunkParams p) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if ((smem_u32(smem) & 1023u) != 0) {  // uniform; checked rather than assumed
+        if (threadIdx.x == 0) atomicOr(p.status, (int)NCKV_ST_TIMEOUT);
+        return;
+    }
+    uint8_t *sQ = smem, *sK = sQ + CH_Q_BYTES, *sV = sK + CH_STAGES * CH_KV_BYTES;
+    // Barriers of key tiles are indexed by the tile's number g in the CTA's stream: stage g % 2 or g % 3, buffer g & 1, and the phase
+    // follows from g as well.  (What each of them says: prefill_attn.cu.)
+    uint64_t *bars = reinterpret_cast<uint64_t *>(sV + CH_VSTAGES * CH_KV_BYTES);
+    uint64_t *bar_q = bars, *bar_k = bars + 1, *bar_v = bars + 3, *bar_s = bars + 6, *bar_o = bars + 8, *bar_p = bars + 10;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 12);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    volatile int *s_poison = reinterpret_cast<volatile int *>(tmem_slot + 2);        // [4]: piece seq (seq & 3) had values that are not finite
+    ChunkStretch *s_stretch = reinterpret_cast<ChunkStretch *>(tmem_slot + 6);       // [CH_PHASES]
+    int *s_bound = reinterpret_cast<int *>(s_stretch + CH_PHASES);                   // [CH_PHASES + 1]: key tiles before a phase
+    int *s_sum = s_bound + CH_PHASES + 1;                                            // [5][6]
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    pdl_wait_prior_grids();
+    if (tid == 0) {
+        prefetch_tensormap(&tmap_q);
+        prefetch_tensormap(&tmap_k);
+        prefetch_tensormap(&tmap_v);
+        mbar_init(bar_q, 1);
+        for (int s = 0; s < CH_STAGES; ++s) mbar_init(&bar_k[s], 1);
+        for (int s = 0; s < CH_VSTAGES; ++s) mbar_init(&bar_v[s], 1);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&bar_s[s], 1);
+            mbar_init(&bar_o[s], 1);
+            mbar_init(&bar_p[s], CH_M / 32);
+        }
+        *abort_flag = 0;
+        for (int i = 0; i < 4; ++i) s_poison[i] = -1;
+        for (int i = 0; i < CH_PHASES; ++i) s_stretch[i].at = s_stretch[i].end = 0;
+        fence_mbar_init();
+    }
+    if (warp == 0) {
+        tmem_alloc(tmem_slot, CH_TMEM_COLS);
+        tmem_relinquish();
+    }
+    // ---- lengths: `width` lanes to a row, a run of rows to each such group of lanes ----------------------
+    int width = 1;
+    while (width < 32 && width < p.n_qtiles) width *= 2;
+    const int member = tid & (width - 1), groups = CH_THREADS / width, group = tid / width;
+    const int run = (p.B + groups - 1) / groups, b_lo = min(group * run, p.B), b_hi = min(b_lo + run, p.B);
+    // key tiles of the row's tiles of queries that this lane counts; per kv head
+    auto my_tiles = [&](const ChunkRow &r, int *longest) {
+        int n = 0;
+        for (int qt = member; qt * p.tile_tokens < r.n; qt += width) {
+            const int c = chunk_span(p, r, qt * p.tile_tokens).count;
+            n += c;
+            if (longest) *longest = max(*longest, c);
+        }
+        return n;
+    };
+    auto row_tiles = [&](const ChunkRow &r) {  // of all the group's lanes
+        int n = my_tiles(r, nullptr);
+        const uint32_t mask = width == 32 ? 0xffffffffu : ((1u << width) - 1) << (lane & ~(width - 1));
+        for (int off = 1; off < width; off <<= 1) n += __shfl_xor_sync(mask, n, off);
+        return n;
+    };
+    int tiles = 0, items = 0, longest = 0, least = 0x7fffffff, most = 0;
+    bool idle = false;  // a row has slots without a token, or can't be
+    for (int b = b_lo; b < b_hi; ++b) {
+        const ChunkRow r = chunk_row(p, b);
+        idle |= r.n < p.T;
+        if (blockIdx.x == 0 && member == 0) {  // lengths out of range: reported once
+            const int L = p.seqlens[b], n = p.new_tokens ? p.new_tokens[b] : p.T;
+            if (L < 0 || n < 0) atomicOr(p.status, (int)NCKV_ST_BAD_SEQLEN);
+            else if (n > p.T || (long long)L + n > p.capacity) atomicOr(p.status, (int)NCKV_ST_OVERFLOW);
+        }
+        const int n = my_tiles(r, &longest);
+        tiles += n * p.Hkv;
+        if (member == 0) items += (r.n + p.tile_tokens - 1) / p.tile_tokens * p.Hkv;
+        if (p.n_qtiles > 1) {
+            const long long work = r.n > 0 ? (long long)chunk_span(p, r, (r.n - 1) / p.tile_tokens * p.tile_tokens).count * r.n : 0;
+            const int last = (int)min(work, 0x7fffffffLL);
+            least = min(least, last);
+            most = max(most, last);
+        }
+    }
+    int before = tiles;  // inclusive sum over the warp, then over the threads before this one
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, before, off);
+        if (lane >= off) before += v;
+    }
+    items = __reduce_add_sync(0xffffffffu, items);
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    least = __reduce_min_sync(0xffffffffu, least);
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 31) {
+        s_sum[warp] = before;
+        s_sum[6 + warp] = items;
+        s_sum[12 + warp] = longest;
+        s_sum[18 + warp] = least;
+        s_sum[24 + warp] = most;
+    }
+    tc_fence_before();
+    const bool any_idle = __syncthreads_or(idle);
+    tc_fence_after();
+    int all = 0;
+    before -= tiles;
+    items = 0;
+    for (int w = 0; w < CH_THREADS / 32; ++w) {
+        if (w < warp) before += s_sum[w];
+        all += s_sum[w];
+        items += s_sum[6 + w];
+        longest = max(longest, s_sum[12 + w]);
+        least = min(least, s_sum[18 + w]);
+        most = max(most, s_sum[24 + w]);
+    }
+    before = __shfl_sync(0xffffffffu, before, lane & ~(width - 1));  // of the group's first lane: tiles before its rows
+    const bool dealt = chunk_dealt(p, least, most, all, items, longest, (int)gridDim.x);
+    if (dealt) {
+        if (blockIdx.x == 0 && tid == 0 && p.phases) p.plan[1] = 0;
+    } else {
+        // where the phases begin, and the places of all tiles for the kernel behind
+        if (tid == 0) s_bound[p.phases] = all;
+        for (int b = b_lo, base = before; b < b_hi; ++b) {
+            const ChunkRow r = chunk_row(p, b);
+            const int n = row_tiles(r);
+            for (int f = 0; f < p.phases; ++f) {
+                const int pair = f * p.phase_pairs - b * p.Hkv;
+                if (member == 0 && pair >= 0 && pair < p.Hkv) s_bound[f] = base + pair * n;
+            }
+            if (b % (int)gridDim.x == (int)blockIdx.x && member == 0) {
+                int32_t *plan = p.plan + CH_PLAN + (long long)b * (p.n_qtiles + 2);
+                plan[0] = base;
+                plan[1] = n;
+                int at = 0;
+                for (int qt = 0; qt * p.tile_tokens < r.n; ++qt) {
+                    plan[2 + qt] = at;
+                    at += chunk_span(p, r, qt * p.tile_tokens).count;
+                }
+            }
+            base += n * p.Hkv;
+        }
+        __syncthreads();
+        for (int f = 0; f < p.phases; ++f) {
+            const int lo = s_bound[f], hi = s_bound[f + 1];
+            const int each = p.phases == 1 && gridDim.x == 1 ? max(hi - lo, 1) : max((hi - lo + (int)gridDim.x - 1) / (int)gridDim.x, CH_MIN_TILES);
+            const int from = (int)min(lo + (long long)each * blockIdx.x, (long long)hi);
+            if (blockIdx.x == 0 && tid == 0) {
+                p.plan[CH_PLAN - 1] = (int)gridDim.x;
+                p.plan[2 * f] = lo;
+                p.plan[2 * f + 1] = each;
+            }
+            if (from >= hi) continue;
+            for (int b = b_lo, base = before; b < b_hi && base <= from; ++b) {
+                const ChunkRow r = chunk_row(p, b);
+                const int n = row_tiles(r), rel = from - base;
+                base += n * p.Hkv;
+                if (from >= base || member) continue;
+                ChunkStretch st;
+                st.at = from;
+                st.end = min(from + each, hi);
+                st.b = b;
+                st.hkv = rel / n;
+                st.off = rel - st.hkv * n;
+                st.qt = 0;
+                for (;; ++st.qt) {
+                    const int count = chunk_span(p, r, st.qt * p.tile_tokens).count;
+                    if (st.off < count) break;
+                    st.off -= count;
+                }
+                s_stretch[f] = st;
+            }
+        }
+    }
+    __syncthreads();
+    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t tmem_s = tmem_base, tmem_o = tmem_base + 128;
+    const uint32_t lane_sel = (uint32_t)((warp & 3) * 32) << 16;  // a warp reaches TMEM lanes 32*(warp % 4) ..
+
+    constexpr uint32_t IDESC_S = umma_idesc(CH_M, CH_N, 0, 0);
+    constexpr uint32_t IDESC_O = umma_idesc(CH_M, NCKV_D, 0, 1);
+    auto timed_out = [&]() {
+        *abort_flag = 1;
+        atomicOr(p.status, (int)NCKV_ST_TIMEOUT);
+    };
+    auto par2 = [](uint32_t g) -> uint32_t { return (g >> 1) & 1u; };
+
+    if (warp == CH_M / 32 + 1) {
+        // =============== one lane moves the tiles ===================================================
+        if (elect_one()) {
+            ChunkCursor kc, vc, wc;  // next K tile, next V tile, tile whose score product is awaited
+            kc.start(p, s_stretch, dealt);
+            vc = kc;
+            wc = kc;
+            uint32_t gk = 0, gv = 0, nq = 0;
+            // Boxes outside [kv_lo, kv_hi) need no page: they read as zeros, as pages outside the pool do.
+            auto load_tile = [&](uint8_t *dst, const CUtensorMap *map, uint64_t *bar, const ChunkCursor &c) {
+                mbar_arrive_expect_tx(bar, CH_KV_BYTES);
+                const int key0 = (c.u.tile0 + c.t) * CH_N;
+                for (int i = 0; i < CH_N; i += p.box) {
+                    const int key = key0 + i, idx = key / p.page_tokens;
+                    int page = p.n_pages;
+                    if (key < c.u.kv_hi && key + p.box > c.u.kv_lo) {
+                        page = __ldg(p.table + (long long)c.u.b * p.max_pages + idx);
+                        if (page < 0 || page >= p.n_pages) {
+                            atomicOr(p.status, (int)NCKV_ST_BAD_PAGE);
+                            page = p.n_pages;
+                        }
+                    }
+                    tma_load_4d(dst + i * 128, map, bar, 0, c.u.hkv, key - idx * p.page_tokens, page);
+                    tma_load_4d(dst + CH_KV_BYTES / 2 + i * 128, map, bar, 64, c.u.hkv, key - idx * p.page_tokens, page);
+                }
+            };
+            auto load_k = [&]() {
+                const int stage = (int)(gk % CH_STAGES);
+                load_tile(sK + stage * CH_KV_BYTES, &tmap_k, &bar_k[stage], kc);
+                kc.advance(p, s_stretch);
+                ++gk;
+            };
+            auto load_v = [&]() {
+                const int stage = (int)(gv % CH_VSTAGES);
+                load_tile(sV + stage * CH_KV_BYTES, &tmap_v, &bar_v[stage], vc);
+                vc.advance(p, s_stretch);
+                ++gv;
+            };
+            auto load_q = [&](const ChunkUnit &u) {
+                mbar_arrive_expect_tx(bar_q, (uint32_t)(p.tile_tokens * p.G * NCKV_D * 2));
+                tma_load_4d(sQ, &tmap_q, bar_q, 0, u.hkv * p.G, u.t0, u.b);
+                tma_load_4d(sQ + CH_Q_BYTES / 2, &tmap_q, bar_q, 64, u.hkv * p.G, u.t0, u.b);
+                ++nq;
+            };
+            bool ok = true;
+            if (wc.valid) {
+                load_q(wc.u);
+                while (gk < CH_STAGES && kc.valid) load_k();
+                while (gv < CH_VSTAGES && vc.valid) load_v();
+                for (uint32_t g = 0; wc.valid && ok; ++g) {
+                    // what S(g)'s completion releases: the Q buffer if g ends its piece, K(g)'s stage for
+                    // K(g+2) and, P V(g-2) being complete too, V(g-2)'s stage for V(g+1)
+                    const bool ends = wc.last_of_unit();
+                    ChunkCursor nx = wc;
+                    nx.advance(p, s_stretch);
+                    if (!kc.valid && !vc.valid && !nx.valid) break;
+                    ok = mbar_wait_bounded(&bar_s[g & 1], par2(g));
+                    if (!ok) break;
+                    if (ends && nx.valid) load_q(nx.u);
+                    if (kc.valid) load_k();
+                    if (vc.valid && gv <= g + 1) load_v();
+                    wc = nx;
+                }
+            }
+            if (!ok) timed_out();
+            if (*abort_flag) {  // the last copies may still be under way
+                if (nq) mbar_wait_bounded(bar_q, (nq - 1) & 1u);
+                for (uint32_t s = 0; s < CH_STAGES && s < gk; ++s) mbar_wait_bounded(&bar_k[(gk - 1 - s) % CH_STAGES], ((gk - 1 - s) / CH_STAGES) & 1u);
+                for (uint32_t s = 0; s < CH_VSTAGES && s < gv; ++s) mbar_wait_bounded(&bar_v[(gv - 1 - s) % CH_VSTAGES], ((gv - 1 - s) / CH_VSTAGES) & 1u);
+            }
+        }
+        __syncwarp();
+    } else if (warp == CH_M / 32) {
+        // =============== one thread feeds the tensor core ==========================================
+        if (elect_one()) {
+            const uint64_t desc_q = smem_desc_sw128(smem_u32(sQ), 16, 1024);
+            const uint64_t desc_k = smem_desc_sw128(smem_u32(sK), 16, 1024);
+            const uint64_t desc_v = smem_desc_sw128(smem_u32(sV), CH_KV_BYTES / 2, 1024);
+            ChunkCursor sc, pc;  // tile of the next score product, tile of the next P V product
+            sc.start(p, s_stretch, dealt);
+            pc = sc;
+            uint32_t gs = 0, gp = 0, n_q = 0;
+            auto issue_s = [&]() -> bool {
+                const uint32_t stage = gs % CH_STAGES;
+                if (sc.t == 0) {  // first tile of a piece: its Q
+                    if (!mbar_wait_bounded(bar_q, n_q & 1u)) return false;
+                    ++n_q;
+                }
+                if (!mbar_wait_bounded(&bar_k[stage], (gs / CH_STAGES) & 1u)) return false;
+                tc_fence_after();
+                const uint64_t dk = desc_k + (uint64_t)((stage * CH_KV_BYTES) >> 4);
+                const uint32_t ds = tmem_s + (gs & 1u) * CH_N;
+#pragma unroll
+                for (int kk = 0; kk < NCKV_D / 16; ++kk) {
+                    const uint32_t off = (uint32_t)(kk & 3) * 32;
+                    const uint64_t da = desc_q + (uint64_t)(((kk >> 2) * (CH_Q_BYTES / 2) + off) >> 4);
+                    const uint64_t db = dk + (uint64_t)(((kk >> 2) * (CH_KV_BYTES / 2) + off) >> 4);
+                    umma_bf16(ds, da, db, IDESC_S, kk > 0 ? 1u : 0u);
+                }
+                umma_commit(&bar_s[gs & 1u]);
+                sc.advance(p, s_stretch);
+                ++gs;
+                return true;
+            };
+            bool ok = true;
+            if (sc.valid) ok = issue_s();
+            if (ok && sc.valid) ok = issue_s();
+            while (pc.valid && ok) {
+                // P(gp) is in TMEM, S(gp) has been read, O carries the scale P was made with
+                const uint32_t vstage = gp % CH_VSTAGES;
+                ok = mbar_wait_bounded(&bar_p[gp & 1u], par2(gp)) && mbar_wait_bounded(&bar_v[vstage], (gp / CH_VSTAGES) & 1u);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t dv = desc_v + (uint64_t)((vstage * CH_KV_BYTES) >> 4);
+                const uint32_t pbase = tmem_s + (gp & 1u) * CH_N;
+#pragma unroll
+                for (int ks = 0; ks < CH_N / 16; ++ks) {
+                    const uint64_t db = dv + (uint64_t)((ks * 16 * 128) >> 4);
+                    umma_bf16_a_tmem(tmem_o, pbase + (uint32_t)ks * 8, db, IDESC_O, (pc.t > 0 || ks > 0) ? 1u : 0u);
+                }
+                const int from_end = pc.u.n_tiles - 1 - pc.t;
+                if (from_end < 2) umma_commit(&bar_o[from_end]);
+                if (sc.valid) ok = issue_s();
+                pc.advance(p, s_stretch);
+                ++gp;
+            }
+            if (!ok) timed_out();
+        }
+        __syncwarp();
+    } else {
+        // =============== softmax threads: one per query row =========================================
+        const int row = tid, tok = row / p.G, head = row - tok * p.G;
+        if (any_idle) {  // zeros, a share of the slots per CTA
+            for (int b = 0; b < p.B; ++b) {
+                const int n = chunk_row(p, b).n;
+                if (n == p.T) continue;
+                const long long words = (long long)(p.T - n) * p.Hq * (NCKV_D / 8);
+                uint4 *dst = reinterpret_cast<uint4 *>(p.out + ((long long)b * p.T + n) * p.Hq * NCKV_D);
+                for (long long i = (long long)blockIdx.x * CH_M + tid; i < words; i += (long long)gridDim.x * CH_M) dst[i] = make_uint4(0, 0, 0, 0);
+            }
+        }
+        bool aborted = false;
+        uint32_t g = 0;               // number of the current piece's tile 0 in the stream
+        uint32_t n_o0 = 0, n_o1 = 0;  // phases of bar_o[0] / bar_o[1] used up by the pieces before this one
+        auto warp_wait = [&](uint64_t *bar, uint32_t parity) -> bool {
+            if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+            int ok = *abort_flag == 0;
+            if (lane == 0 && ok) ok = mbar_wait_bounded(bar, parity) ? 1 : 0;
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            __syncwarp();  // orders the lanes' later reads of the tile behind lane 0's observation
+            return ok != 0;
+        };
+        ChunkCursor cur;
+        for (cur.start(p, s_stretch, dealt); cur.valid && !aborted; cur.load(p, s_stretch)) {
+            const ChunkUnit &it = cur.u;
+            const int n_tiles = it.n_tiles, first_pos = it.L + it.t0, tokens = min(p.tile_tokens, it.n - it.t0);
+            const int pos = first_pos + tok;  // absolute position of this row's token
+            const bool live = tok < tokens;
+            const bool warp_live = warp * 32 < tokens * p.G;  // the other warps only keep the barriers going
+            auto pv_done = [&](int t) -> bool {
+                const int from_end = n_tiles - 1 - t;
+                const uint32_t x = g + (uint32_t)t;
+                return from_end >= 2 ? warp_wait(&bar_s[(x + 2) & 1u], par2(x + 2)) : warp_wait(&bar_o[from_end], (from_end == 0 ? n_o0 : n_o1) & 1u);
+            };
+            // P is scaled by m_used, which follows the running maximum lazily: it is only raised (and the O row in TMEM
+            // rescaled) when the maximum has grown by more than 2^8
+            float m_used = -INFINITY, l_run = 0.f;
+            for (int t = 0; t < n_tiles; ++t) {
+                const uint32_t gt = g + (uint32_t)t;
+                const int key0 = (it.tile0 + t) * CH_N;
+                const uint32_t tmem_s_it = tmem_s + (uint32_t)(gt & 1) * CH_N;
+                if (!warp_wait(&bar_s[gt & 1u], par2(gt))) {  // uniform over the warp
+                    aborted = true;
+                    break;
+                }
+                tc_fence_after();
+                // tiles that some row of the piece doesn't see all of (uniform over the CTA)
+                const bool edge = key0 + CH_N - 1 > first_pos || key0 < it.kv_lo ||
+                                  (p.window_left >= 0 && key0 < first_pos + tokens - 1 - p.window_left);
+                if (warp_live) {
+                    float s_val[CH_N];
+                    tmem_ld64(tmem_s_it + lane_sel, s_val);
+                    if (edge) {
+                        // this row sees columns [c_lo, c_hi) of the tile
+                        const int c_hi = min(pos, it.kv_hi - 1) - key0 + 1;
+                        const int c_lo = p.window_left >= 0 ? pos - p.window_left - key0 : 0;
+#pragma unroll
+                        for (int c = 0; c < CH_N; ++c) s_val[c] = (c >= c_lo && c < c_hi) ? s_val[c] : -INFINITY;
+                    }
+                    float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int c = 0; c < CH_N; c += 8) {
+                        mx4[0] = fmax3(mx4[0], s_val[c], s_val[c + 1]);
+                        mx4[1] = fmax3(mx4[1], s_val[c + 2], s_val[c + 3]);
+                        mx4[2] = fmax3(mx4[2], s_val[c + 4], s_val[c + 5]);
+                        mx4[3] = fmax3(mx4[3], s_val[c + 6], s_val[c + 7]);
+                    }
+                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
+                    const bool raise = mx > m_used + 8.f;  // also the first tile that shows this row a key (m_used = -inf)
+                    const float alpha = raise ? ex2_approx(m_used - mx) : 1.f;
+                    if (raise) {
+                        l_run *= alpha;
+                        m_used = mx;
+                    }
+                    const float m_use = m_used == -INFINITY ? 0.f : m_used;  // a row that has seen no key yet
+                    float2 rs01 = make_float2(0.f, 0.f), rs23 = make_float2(0.f, 0.f);
+                    const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), neg_m2 = make_float2(-m_use, -m_use);
+                    uint32_t pk[CH_N / 2];
+#pragma unroll
+                    for (int c = 0; c < CH_N; c += 4) {
+                        const float2 x01 = ffma2(make_float2(s_val[c], s_val[c + 1]), scale2, neg_m2);
+                        const float2 x23 = ffma2(make_float2(s_val[c + 2], s_val[c + 3]), scale2, neg_m2);
+                        const float2 p01 = make_float2(ex2_approx(x01.x), ex2_approx(x01.y));
+                        const float2 p23 = make_float2(ex2_approx(x23.x), ex2_approx(x23.y));
+                        rs01 = fadd2(rs01, p01);
+                        rs23 = fadd2(rs23, p23);
+                        pk[c / 2] = pack_bf16x2(p01.x, p01.y);
+                        pk[c / 2 + 1] = pack_bf16x2(p23.x, p23.y);
+                    }
+                    l_run += (rs01.x + rs01.y) + (rs23.x + rs23.y);
+                    tmem_st_words(tmem_s_it + lane_sel, pk);
+                    if (t > 0 && __any_sync(0xffffffffu, raise)) {
+                        if (!pv_done(t - 1)) {
+                            timed_out();
+                            aborted = true;
+                            break;
+                        }
+                        tc_fence_after();
+#pragma unroll
+                        for (int ch = 0; ch < NCKV_D / 32; ++ch) {
+                            float c[32];
+                            tmem_ld32(tmem_o + lane_sel + ch * 32, c);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) c[i] *= alpha;
+                            tmem_st32(tmem_o + lane_sel + ch * 32, c);
+                        }
+                    }
+                }
+                if (edge) {
+                    // Keys that nobody of the piece sees may hold anything, keys that only some rows see may hold values that are not
+                    // finite: a probability of zero must meet neither.
+                    const int stage = (int)(gt % CH_VSTAGES), lo = it.kv_lo - key0, hi = it.kv_hi - key0;
+                    uint8_t *vd = sV + stage * CH_KV_BYTES;
+                    if (warp_wait(&bar_v[stage], (gt / CH_VSTAGES) & 1u)) {
+#pragma unroll 2
+                        for (int i = tid; i < CH_N * 16; i += CH_M) {
+                            const int r = i >> 4, ch = i & 15;
+                            uint4 *w = reinterpret_cast<uint4 *>(vd + (ch >> 3) * (CH_KV_BYTES / 2) + r * 128 + ((ch & 7) << 4));
+                            if (r < lo || r >= hi) {
+                                *w = make_uint4(0, 0, 0, 0);
+                                continue;
+                            }
+                            uint4 x = *w;
+                            if (not_finite2(x.x) | not_finite2(x.y) | not_finite2(x.z) | not_finite2(x.w)) {
+                                uint16_t *e = reinterpret_cast<uint16_t *>(w);
+                                for (int k = 0; k < 8; ++k)
+                                    if ((e[k] & 0x7f80u) == 0x7f80u) e[k] = 0;
+                                s_poison[cur.seq & 3] = cur.seq;
+                            }
+                        }
+                    }
+                    fence_proxy_async_smem();  // the cleared values must be visible to the tensor core
+                }
+                tc_fence_before();  // orders this thread's TMEM loads/stores before the next MMAs
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar_p[gt & 1]);  // one arrival per warp
+            }
+            if (aborted) break;
+
+            // ---- the piece's end ---------------------------------------------------------------------
+            if (!pv_done(n_tiles - 1)) {
+                timed_out();
+                aborted = true;
+                break;
+            }
+            tc_fence_after();
+            if (warp_live) {
+                const bool poison = s_poison[cur.seq & 3] == cur.seq;
+                const float inv = it.slot >= 0 ? 1.f : (l_run > 0.f ? 1.f / l_run : (l_run == l_run ? 0.f : l_run));
+                const long long part = (long long)it.slot * p.part_rows + row;
+                uint4 *dst = reinterpret_cast<uint4 *>(p.out + (((long long)it.b * p.T + it.t0 + tok) * p.Hq + it.hkv * p.G + head) * NCKV_D);
+                if (it.slot >= 0 && live) *reinterpret_cast<float2 *>(p.part_ml + part * 2) = make_float2(m_used, l_run);
+#pragma unroll
+                for (int ch = 0; ch < NCKV_D / 32; ++ch) {
+                    float c[32];
+                    __syncwarp();
+                    tmem_ld32(tmem_o + lane_sel + ch * 32, c);
+                    if (live) {
+                        if (poison) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) c[i] += chunk_not_finite(p, it, pos, ch * 32 + i);
+                        }
+                        if (it.slot >= 0) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                uint32_t w[8];
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(c[8 * i + e]);
+                                st_global_v8(p.part_o + part * NCKV_D + ch * 32 + i * 8, w);
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {  // 32 bytes per store: whole sectors
+                                uint32_t w[8];
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) w[e] = pack_bf16x2(c[16 * i + 2 * e] * inv, c[16 * i + 2 * e + 1] * inv);
+                                st_global_v8(dst + (ch * 2 + i) * 2, w);
+                            }
+                        }
+                    }
+                }
+                __syncwarp();
+            }
+            // O is read: order those loads before the first P V of the next piece, which overwrites it and
+            // is only issued after this thread's next arrival on bar_p
+            tc_fence_before();
+            g += (uint32_t)n_tiles;
+            n_o0 += 1;
+            n_o1 += n_tiles >= 2;
+        }
+        if (aborted && *abort_flag == 0) timed_out();  // a wait ran out in this warp
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) tmem_dealloc(tmem_base, CH_TMEM_COLS);
+}
+
+// Adds up the parts of every query row whose keys were cut: O = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s.  WARPS warps to a row.
+template <int WARPS>
+__global__ void __launch_bounds__(256) chunk_finish_kernel(const __grid_constant__ ChunkParams p) {
+    pdl_wait_prior_grids();
+    constexpr int ROWS = 8 / WARPS;
+    __shared__ float4 s_o[8][32];
+    __shared__ float2 s_ml[8];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = warp % WARPS;
+    if (p.plan[1] == 0) return;  // dealt
+    const int grid = p.plan[CH_PLAN - 1];
+    const long long n_rows = (long long)p.B * p.T * p.Hq;
+    for (long long r0 = (long long)blockIdx.x * ROWS; r0 < n_rows; r0 += (long long)gridDim.x * ROWS) {
+        const long long at = r0 + warp / WARPS;
+        // the tile's key tiles begin at `from`; its parts lie in the slots of `count` CTAs from `first` on, whose stretches begin at begin + c each
+        int first = 0, count = 0, from = 0, begin = 0, each = 1, phase = 0, in_unit = 0;
+        if (at < n_rows) {
+            const int hq = (int)(at % p.Hq), t = (int)(at / p.Hq % p.T), b = (int)(at / p.Hq / p.T);
+            const int hkv = hq / p.G, qt = t / p.tile_tokens;
+            const ChunkRow r = chunk_row(p, b);
+            in_unit = (t - qt * p.tile_tokens) * p.G + hq - hkv * p.G;
+            if (t < r.n) {
+                const int32_t *plan = p.plan + CH_PLAN + (long long)b * (p.n_qtiles + 2);
+                const int tiles = chunk_span(p, r, qt * p.tile_tokens).count;
+                phase = (b * p.Hkv + hkv) / p.phase_pairs;
+                begin = p.plan[2 * phase];
+                each = p.plan[2 * phase + 1];
+                from = plan[0] + hkv * plan[1] + plan[2 + qt];
+                first = (from - begin) / each;
+                count = (from - begin + tiles - 1) / each - first + 1;
+                if (count == 1) count = 0;  // written already
+            }
+        }
+        auto part_of = [&](int i) -> long long {  // row of part i
+            const int c = first + i;
+            const long long slot = ((long long)phase * grid + c) * 2 + (begin + c * each < from);  // + 1: not the first piece of the stretch
+            return slot * p.part_rows + in_unit;
+        };
+        float m = -INFINITY, l = 0.f;
+        for (int i = lane; i < count; i += 32) {
+            m = fmaxf(m, p.part_ml[part_of(i) * 2]);
+        }
+#pragma unroll
+        for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int i = mine; i < count; i += WARPS) {
+            const long long at_part = part_of(i);
+            const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + at_part * 2);
+            const float4 x = reinterpret_cast<const float4 *>(p.part_o + at_part * NCKV_D)[lane];
+            if (ml.x == -INFINITY && ml.y == 0.f) continue;  // this row sees none of the part's keys
+            const float w = exp2f(ml.x - m);
+            l += w * ml.y;
+            o.x += w * x.x;
+            o.y += w * x.y;
+            o.z += w * x.z;
+            o.w += w * x.w;
+        }
+        if (WARPS > 1) {
+            s_o[warp][lane] = o;
+            if (lane == 0) s_ml[warp] = make_float2(m, l);
+            __syncthreads();
+            if (mine == 0) {
+#pragma unroll
+                for (int w = 1; w < WARPS; ++w) {
+                    const float4 x = s_o[warp + w][lane];
+                    l += s_ml[warp + w].y;
+                    o.x += x.x;
+                    o.y += x.y;
+                    o.z += x.z;
+                    o.w += x.w;
+                }
+            }
+            __syncthreads();
+        }
+        if (mine == 0 && count) {
+            const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+            reinterpret_cast<uint2 *>(p.out + at * NCKV_D)[lane] = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+        }
+    }
+}
+
+static size_t chunk_smem_bytes() { return CH_Q_BYTES + (CH_STAGES + CH_VSTAGES) * CH_KV_BYTES + 12 * sizeof(uint64_t) + (2 + 4 + 6 * CH_PHASES + CH_PHASES + 1 + 30) * 4; }
+
+// How a launch of these sizes is cut: what of it doesn't depend on the rows' lengths.
+struct ChunkShape {
+    int G, tile_tokens, n_qtiles, grid, phases, phase_pairs, part_rows;
+    long long n_items;
+    size_t plan_bytes;
+};
+static ChunkShape chunk_shape(int B, int T, int Hq, int Hkv, long long capacity, long long window_left) {
+    ChunkShape s;
+    s.G = Hq / Hkv;
+    s.tile_tokens = CH_M / s.G < T ? CH_M / s.G : T;
+    s.n_qtiles = (T + s.tile_tokens - 1) / s.tile_tokens;
+    s.n_items = (long long)B * Hkv * s.n_qtiles;
+    s.part_rows = s.tile_tokens * s.G;
+    const int most = 2 * sm_count();  // two CTAs per SM
+    const long long key_tiles = (capacity + CH_N - 1) / CH_N, pairs = (long long)B * Hkv;
+    s.grid = (int)(s.n_items * key_tiles < most ? s.n_items * key_tiles : most);
+    long long keys = window_left >= 0 && window_left + T < capacity ? window_left + T : capacity;
+    s.phases = 1;
+    if (s.n_qtiles > 1) {
+        long long n = (pairs * keys * 512 + CH_PHASE_BYTES - 1) / CH_PHASE_BYTES;
+        const long long room = CH_PART_BYTES / ((long long)2 * s.grid * s.part_rows * (NCKV_D + 2) * 4);
+        n = n < room ? n : room;
+        n = n < pairs ? n : pairs;
+        s.phases = (int)(n < 1 ? 1 : n < CH_PHASES ? n : CH_PHASES);
+    }
+    s.phase_pairs = (int)((pairs + s.phases - 1) / s.phases);
+    s.phases = (int)((pairs + s.phase_pairs - 1) / s.phase_pairs);
+    if (s.grid == 1) s.phases = 0;
+    s.plan_bytes = ((size_t)(CH_PLAN + (size_t)B * (s.n_qtiles + 2)) * 4 + 255) / 256 * 256;
+    return s;
+}
+static size_t chunk_workspace(const ChunkShape &s) {
+    return s.phases ? s.plan_bytes + (size_t)s.phases * 2 * s.grid * s.part_rows * (NCKV_D + 2) * 4 : 0;
+}
+static int chunk_check_sizes(const char *name, int B, int T, int Hq, int Hkv, int page_tokens, int max_pages) {
+    if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || page_tokens <= 0 || max_pages <= 0) {
+        set_error("%s: non-positive size (B=%d T=%d Hq=%d Hkv=%d page_tokens=%d max_pages=%d)", name, B, T, Hq, Hkv, page_tokens, max_pages);
+        return NCKV_E_ARG;
+    }
+    if (Hq % Hkv != 0 || Hq / Hkv > CH_M) {
+        set_error("%s: Hq=%d must be a multiple of Hkv=%d, at most %d times it", name, Hq, Hkv, CH_M);
+        return NCKV_E_UNSUPPORTED;
+    }
+    if (page_tokens % nckv_paged_tile_tokens() != 0) {
+        set_error("%s: page_tokens=%d must be a multiple of %d", name, page_tokens, nckv_paged_tile_tokens());
+        return NCKV_E_ARG;
+    }
+    const long long capacity = (long long)page_tokens * max_pages;
+    const long long key_tiles = (capacity + CH_N - 1) / CH_N, pairs = (long long)B * Hkv;
+    if (capacity > 0x3fffffffLL || pairs > 0x3fffffffLL || pairs * T > 0x3fffffffLL ||
+        pairs * ((T + CH_M / (Hq / Hkv) - 1) / (CH_M / (Hq / Hkv))) > 0x3fffffffLL / key_tiles) {
+        set_error("%s: B=%d T=%d Hkv=%d with %lld tokens of capacity is too large for one launch", name, B, T, Hkv, capacity);
+        return NCKV_E_UNSUPPORTED;
+    }
+    return NCKV_OK;
+}
+
+}  // namespace nckv
+
+extern "C" size_t nckv_prefill_attn_paged_workspace_bytes(int B, int T, int Hq, int Hkv, int page_tokens, int max_pages, int window_left) {
+    using namespace nckv;
+    if (chunk_check_sizes("prefill_attn_paged_workspace_bytes", B, T, Hq, Hkv, page_tokens, max_pages) != NCKV_OK) return 0;
+    return chunk_workspace(chunk_shape(B, T, Hq, Hkv, (long long)page_tokens * max_pages, window_left));
+}
+
+extern "C" int nckv_prefill_attn_paged(const void *q, const void *k_pool, const void *v_pool, const int32_t *block_table,
+                                       const int32_t *cache_seqlens, const int32_t *new_tokens, void *out, int B, int T, int Hq, int Hkv,
+                                       int D, int page_tokens, int max_pages, int n_pages, int64_t page_stride, int64_t token_stride,
+                                       int window_left, void *workspace, size_t workspace_bytes, int32_t *status, void *stream) {
+    using namespace nckv;
+    const char *name = "prefill_attn_paged";
+    if (!q || !k_pool || !v_pool || !block_table || !cache_seqlens || !out || !status) {
+        set_error("%s: null pointer argument", name);
+        return NCKV_E_ARG;
+    }
+    if (D != NCKV_D) {
+        set_error("%s: head_dim %d unsupported (kernels are built for 128)", name, D);
+        return NCKV_E_UNSUPPORTED;
+    }
+    int rc = chunk_check_sizes(name, B, T, Hq, Hkv, page_tokens, max_pages);
+    if (rc != NCKV_OK) return rc;
+    if (n_pages <= 0 || page_stride < 0) {
+        set_error("%s: n_pages=%d must be positive", name, n_pages);
+        return NCKV_E_ARG;
+    }
+    if (((uintptr_t)q & 15) || ((uintptr_t)out & 31)) {
+        set_error("%s: q must be 16-byte and out 32-byte aligned", name);
+        return NCKV_E_ARG;
+    }
+    const ChunkShape s = chunk_shape(B, T, Hq, Hkv, (long long)page_tokens * max_pages, window_left);
+    const size_t need = chunk_workspace(s);
+    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))) {
+        set_error("%s: needs %zu bytes of workspace, 256-byte aligned", name, need);
+        return workspace && workspace_bytes < need ? NCKV_E_CAPACITY : NCKV_E_ARG;
+    }
+    int box = CH_N;
+    while (page_tokens % box) box /= 2;  // 16 at least: pages are multiples of 48
+    CUtensorMap mq, mk, mv;
+    const int64_t dims[4] = {D, Hq, T, B}, strides[3] = {D, (int64_t)Hq * D, (int64_t)T * Hq * D};
+    const int q_box[4] = {64, s.G, s.tile_tokens, 1};
+    rc = make_tensor_map(&mq, q, 4, dims, strides, q_box);
+    if (rc != NCKV_OK) return rc;
+    rc = make_kv_tensor_map(&mk, k_pool, n_pages, page_tokens, Hkv, page_stride, token_stride, box);
+    if (rc != NCKV_OK) return rc;
+    rc = make_kv_tensor_map(&mv, v_pool, n_pages, page_tokens, Hkv, page_stride, token_stride, box);
+    if (rc != NCKV_OK) return rc;
+
+    ChunkParams p;
+    p.table = block_table;
+    p.seqlens = cache_seqlens;
+    p.new_tokens = new_tokens;
+    p.v_pool = static_cast<const __nv_bfloat16 *>(v_pool);
+    p.out = static_cast<__nv_bfloat16 *>(out);
+    p.plan = static_cast<int32_t *>(workspace);
+    p.part_o = p.part_ml = nullptr;
+    if (s.phases) {
+        p.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + s.plan_bytes);
+        p.part_ml = p.part_o + (size_t)s.phases * 2 * s.grid * s.part_rows * NCKV_D;
+    }
+    p.status = status;
+    p.B = B; p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.G = s.G; p.tile_tokens = s.tile_tokens; p.n_qtiles = s.n_qtiles;
+    p.page_tokens = page_tokens; p.max_pages = max_pages; p.n_pages = n_pages; p.capacity = page_tokens * max_pages; p.box = box;
+    p.page_stride = page_stride; p.token_stride = token_stride;
+    p.window_left = window_left;
+    p.phases = s.phases; p.phase_pairs = s.phase_pairs; p.part_rows = s.part_rows;
+    p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)D));
+    {
+        // Pairs per group: all of them while their keys and values fit a third of L2, else as many as do, rounded down to a
+        // number whose tiles are a multiple of two rounds of the CTAs (dealt back and forth, every CTA then gets the same mix).
+        const long long keys = window_left >= 0 && (long long)window_left + CH_M < p.capacity ? window_left + CH_M : p.capacity;
+        const long long pairs = (long long)B * Hkv, bytes_per_pair = keys * 512 + 1;
+        long long g = pairs;
+        if (pairs * bytes_per_pair > (40LL << 20)) {
+            g = (40LL << 20) / bytes_per_pair;
+            long long a = 2LL * s.grid, b = s.n_qtiles;
+            while (b) { const long long t = a % b; a = b; b = t; }
+            const long long unit = 2LL * s.grid / a;  // pairs
+            if (g >= unit) g -= g % unit;
+            if (g < 1) g = 1;
+            if (g > pairs) g = pairs;
+        }
+        p.n_groups = (int)(pairs / g);  // the last group also takes the remainder
+        p.group_pairs = (int)g;
+    }
+    const size_t smem = chunk_smem_bytes();
+    static bool attr_set[64] = {false};
+    int dev = 0;
+    NCKV_CUDA_CHECK(cudaGetDevice(&dev));
+    if (dev >= 64 || !attr_set[dev]) {
+        NCKV_CUDA_CHECK(cudaFuncSetAttribute(chunk_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        if (dev < 64) attr_set[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)s.grid);
+    cfg.blockDim = dim3(CH_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    NCKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, chunk_attn_kernel, mq, mk, mv, p));
+    if (s.phases) {
+        const long long rows = (long long)B * T * Hq, most = 8LL * sm_count();
+        const bool wide = rows <= 2LL * sm_count();
+        const long long blocks = wide ? rows : (rows + 7) / 8;
+        cfg.gridDim = dim3((unsigned)(blocks < most ? blocks : most));
+        cfg.blockDim = dim3(256);
+        cfg.dynamicSmemBytes = 0;
+        NCKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, wide ? chunk_finish_kernel<8> : chunk_finish_kernel<1>, p));
+    }
+    return NCKV_OK;
+}

@@ -50,7 +50,7 @@ def compute_window_sizes(sequence_len, n_layer, window_pattern="SSSL"):
     return sizes
 
 
-def kv_attention(q, k, v, cos_sin_tables, window_size, kv_cache, layer_idx):
+def kv_attention(q, k, v, cos_sin_tables, window_size, kv_cache, layer_idx, new_tokens=None):
     """The KV-cache branch of CausalSelfAttention.forward (gpt.py:97-121) in two launches, or one (few rows, short caches).
 
     q: (B, T, Hq, D), k, v: (B, T, Hkv, D) straight from the projections (v already carries the
@@ -59,6 +59,8 @@ def kv_attention(q, k, v, cos_sin_tables, window_size, kv_cache, layer_idx):
     ``get_pos()`` synchronisation and no table slicing is needed.  Launch 1 applies RoPE, QK-norm
     and the 1.2 scale to q and k and appends k/v to the layer's cache; launch 2 attends.
     As in the reference the cache position is advanced once, after the last layer.
+    Over a paged cache (whose pages the caller has reserved) ``new_tokens`` (int32 per row) says how many of a row's T slots
+    hold a token: the others leave the cache alone, their outputs are zero, and each row advances by its own count.
     Returns y of shape (B, T, Hq, D).
     """
     cos, sin = cos_sin_tables
@@ -69,23 +71,25 @@ def kv_attention(q, k, v, cos_sin_tables, window_size, kv_cache, layer_idx):
     left = left if left >= 0 else -1
     paged = getattr(kv_cache, "paged", False)
     call = (q, k, v, k_cache, v_cache, kv_cache.block_table if paged else None, seqlens, cos, sin, left)
-    y = ops.append_and_attend(*call)
-    if y is None and T == 1:
+    y = ops.append_and_attend(*call) if new_tokens is None else None
+    if y is None and T == 1 and new_tokens is None:
         y = ops.append_and_attend_small(*call)
     if y is not None:
         if layer_idx == kv_cache.n_layers - 1:
             kv_cache.advance(T)
         return y
     if paged:  # page pools + block table instead of dense rows
-        if T != 1:
-            raise NotImplementedError("a paged cache takes one new token per row; prefill the prompt into a dense "
-                                      "batch-1 KVCache and hand it over with PagedKVCache.prefill")
-        q2 = ops.append_rope_norm_paged(q, k, v, k_cache, v_cache, kv_cache.block_table, seqlens, cos, sin)
-        y = ops.decode_attention_paged(q2[:, 0], k_cache, v_cache, kv_cache.block_table, seqlens, seqlen_offset=1,
-                                       window_left=left).unsqueeze(1)
+        q2 = ops.append_rope_norm_paged(q, k, v, k_cache, v_cache, kv_cache.block_table, seqlens, cos, sin, new_tokens=new_tokens)
+        if T == 1 and new_tokens is None:
+            y = ops.decode_attention_paged(q2[:, 0], k_cache, v_cache, kv_cache.block_table, seqlens, seqlen_offset=1,
+                                           window_left=left).unsqueeze(1)
+        else:
+            y = ops.prefill_attention_paged(q2, k_cache, v_cache, kv_cache.block_table, seqlens, new_tokens, left)
         if layer_idx == kv_cache.n_layers - 1:
-            kv_cache.advance(T)
+            kv_cache.advance(T if new_tokens is None else new_tokens)
         return y
+    if new_tokens is not None:
+        raise NotImplementedError("counts of new tokens per row need a paged cache")
     q2 = ops.append_rope_norm(q, k, v, k_cache, v_cache, seqlens, cos, sin)
     if T == 1:
         y = ops.decode_attention(q2[:, 0], k_cache, v_cache, seqlens, seqlen_offset=1, window_left=left).unsqueeze(1)

@@ -677,11 +677,20 @@ def _pool_strides(name, pool, table, B):
     return pool.stride(0), pool.stride(1)
 
 
-def append_rope_norm_paged(q, k, v, k_pool, v_pool, block_table, cache_seqlens, cos, sin, qk_scale=QK_SCALE, eps=RMS_EPS):
+def _check_counts(name, new_tokens, B, device):
+    if new_tokens is not None and (new_tokens.dtype != torch.int32 or new_tokens.device != device or new_tokens.shape != (B,) or
+                                   not new_tokens.is_contiguous()):
+        raise RuntimeError(f"nckv::{name}: new_tokens must be a contiguous int32 tensor of {B} rows on {device}")
+
+
+def append_rope_norm_paged(q, k, v, k_pool, v_pool, block_table, cache_seqlens, cos, sin, qk_scale=QK_SCALE, eps=RMS_EPS,
+                           new_tokens=None):
     """``append_rope_norm`` into paged storage: k/v of row b's token at position p go to page
-    ``block_table[b, p // page_tokens]``.  Returns q'."""
+    ``block_table[b, p // page_tokens]``.  Returns q'.  With ``new_tokens`` (int32 per row) only the first
+    ``new_tokens[b]`` of a row's slots hold a token: the others write nothing, and q' is zero there."""
     name = "append_rope_norm_paged"
     _require_cuda(name, q, k, v, k_pool, v_pool, cache_seqlens, cos, sin)
+    _check_counts(name, new_tokens, q.size(0), q.device)
     _require_bf16(name, q, k, v, k_pool, v_pool, cos, sin)
     if cache_seqlens.dtype != torch.int32:
         raise RuntimeError(f"nckv::{name}: cache_seqlens must be int32")
@@ -699,8 +708,9 @@ def append_rope_norm_paged(q, k, v, k_pool, v_pool, block_table, cache_seqlens, 
     q_out = torch.empty_like(q)
     idx, stream, ws = _launch_ctx(q, B, Hq, Hkv)
     with _device_guard(idx):
-        _lib.call("nckv_append_rope_norm_paged", q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(),
-                  k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(), cache_seqlens.data_ptr(), cos2.data_ptr(),
+        _lib.call("nckv_append_rope_norm_paged_counts", q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(),
+                  k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(), cache_seqlens.data_ptr(),
+                  new_tokens.data_ptr() if new_tokens is not None else None, cos2.data_ptr(),
                   sin2.data_ptr(), B, T_new, Hq, Hkv, D, k_pool.size(1), block_table.size(1), k_pool.size(0), sp, st,
                   cos2.size(0), qk_scale, eps, ws.data_ptr(), stream)
     return q_out
@@ -727,6 +737,46 @@ def decode_attention_paged(q, k_pool, v_pool, block_table, cache_seqlens, seqlen
         _lib.call("nckv_decode_attn_paged", q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(),
                   cache_seqlens.data_ptr(), out.data_ptr(), None, None, B, Hq, Hkv, D, k_pool.size(1), block_table.size(1),
                   k_pool.size(0), sp, st, seqlen_offset, window_left, ws.data_ptr(), ws.numel(), stream)
+    return out
+
+
+def prefill_attention_paged(q, k_pool, v_pool, block_table, cache_seqlens, new_tokens=None, window_left=-1):
+    """``prefill_attention`` over paged storage that holds the new keys already: q (B, T, Hq, D), row b's queries at
+    positions ``cache_seqlens[b] + t``.  With ``new_tokens`` (int32 per row) only the first ``new_tokens[b]`` of a row's T
+    slots hold a token; the output is zero in the others."""
+    name = "prefill_attn_paged"
+    _require_cuda(name, q, k_pool, v_pool, block_table, cache_seqlens, new_tokens)
+    _require_bf16(name, q, k_pool, v_pool)
+    if q.dim() != 4 or q.size(3) != HEAD_DIM:
+        raise RuntimeError(f"nckv::{name}: q must be (B, T, Hq, {HEAD_DIM}), got {tuple(q.shape)}")
+    B, T, Hq, D = q.shape
+    if any(t.device != q.device for t in (k_pool, v_pool, block_table, cache_seqlens)):
+        raise RuntimeError(f"nckv::{name}: all tensors must be on {q.device}")
+    if cache_seqlens.dtype != torch.int32 or cache_seqlens.shape != (B,) or not cache_seqlens.is_contiguous():
+        raise RuntimeError(f"nckv::{name}: cache_seqlens must be a contiguous int32 tensor of {B} rows")
+    _check_counts(name, new_tokens, B, q.device)
+    sp, st = _pool_strides(name, k_pool, block_table, B)
+    Hkv = k_pool.size(2)
+    if k_pool.shape != v_pool.shape or k_pool.stride() != v_pool.stride() or Hkv == 0 or Hq % Hkv:
+        raise RuntimeError(f"nckv::{name}: pools {tuple(k_pool.shape)} / {tuple(v_pool.shape)} do not fit q {tuple(q.shape)}")
+    window_left = max(-1, min(int(window_left), 1 << 30))
+    q = q.contiguous()
+    if q.data_ptr() % 16:
+        q = q.clone()
+    out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
+    if out.numel() == 0:
+        return out
+    status = workspace(q.device, 1, 1, 1)
+    idx = q.device.index
+    stream = torch.cuda.current_stream(idx).cuda_stream
+    with _device_guard(idx):
+        need = _lib.lib.nckv_prefill_attn_paged_workspace_bytes(B, T, Hq, Hkv, k_pool.size(1), block_table.size(1), window_left)
+        # partial sums and where they lie: the call's own (or the graph's that holds it)
+        scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        _lib.call("nckv_prefill_attn_paged", q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(),
+                  cache_seqlens.data_ptr(), new_tokens.data_ptr() if new_tokens is not None else None, out.data_ptr(), B, T, Hq, Hkv, D,
+                  k_pool.size(1), block_table.size(1), k_pool.size(0), sp, st, window_left, scratch.data_ptr() if need else None, need,
+                  status.data_ptr(), stream)
     return out
 
 
