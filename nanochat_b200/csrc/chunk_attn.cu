@@ -36,15 +36,18 @@ constexpr int CH_Q_BYTES = CH_M * NCKV_D * 2, CH_KV_BYTES = CH_N * NCKV_D * 2;
 constexpr int CH_TMEM_COLS = 256;  // S / P buffers [0, 64), [64, 128); O [128, 256)
 constexpr int CH_PHASES = 4;       // most groups of pairs that are cut one after the other
 constexpr int CH_MIN_TILES = 1;    // shortest stretch of a CTA
-constexpr int CH_PLAN = 16;        // words of the plan ahead of the tiles' places: begin and stretch of every phase, and its number of stretches
+constexpr int CH_RING = 8;         // pieces of work that the copying thread can be ahead with: it is four at most (five stages, pieces of one tile)
 constexpr long long CH_PART_BYTES = 160LL << 20, CH_PHASE_BYTES = 48LL << 20;
+
+struct ChunkPlan {  // a CTA's stretch of a phase: its first key tile (-1: none), how far into which tile of queries that is, and the whole tile's key tiles
+    int at, off, count, b, hkv, t0, begin, each;  // the phase begins at `begin` and is cut every `each`
+};
 
 struct ChunkParams {
     const int32_t *table, *seqlens, *new_tokens;  // new_tokens may be null: T for every row
     const __nv_bfloat16 *v_pool;
     __nv_bfloat16 *out;
-    int32_t *plan;   // [2 f], [2 f + 1]: first key tile and stretch of phase f (0: dealt); from CH_PLAN on, for every row: key tiles before it,
-                     // key tiles per kv head, then key tiles before each of its tiles of queries
+    ChunkPlan *plan; // (phases, CTAs): how the stretches were cut
     float *part_ml;  // (slots, part_rows, 2): maximum and sum
     float *part_o;   // (slots, part_rows, 128), not divided by the sum
     int32_t *status;
@@ -245,25 +248,27 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     // Barriers of key tiles are indexed by the tile's number g in the CTA's stream: stage g % 2 or g % 3, buffer g & 1, and the phase
     // follows from g as well.  (What each of them says: prefill_attn.cu.)
     uint64_t *bars = reinterpret_cast<uint64_t *>(sV + CH_VSTAGES * CH_KV_BYTES);
-    uint64_t *bar_q = bars, *bar_k = bars + 1, *bar_v = bars + 3, *bar_s = bars + 6, *bar_o = bars + 8, *bar_p = bars + 10;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 12);
+    uint64_t *bar_q = bars, *bar_k = bars + 2, *bar_v = bars + 4, *bar_s = bars + 7, *bar_o = bars + 9, *bar_p = bars + 11;
+    uint64_t *bar_u = bars + 13;  // [CH_RING] piece posted
+    ChunkUnit *ring = reinterpret_cast<ChunkUnit *>(bars + 13 + CH_RING);            // piece u of the CTA at u % CH_RING; n_tiles 0: no more
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(ring + CH_RING);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     volatile int *s_poison = reinterpret_cast<volatile int *>(tmem_slot + 2);        // [4]: piece seq (seq & 3) had values that are not finite
     ChunkStretch *s_stretch = reinterpret_cast<ChunkStretch *>(tmem_slot + 6);       // [CH_PHASES]
     int *s_bound = reinterpret_cast<int *>(s_stretch + CH_PHASES);                   // [CH_PHASES + 1]: key tiles before a phase
-    int *s_sum = s_bound + CH_PHASES + 1;                                            // [5][6]
+    int *s_sum = reinterpret_cast<int *>(ring);                                      // [5][6], before there are pieces
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    pdl_wait_prior_grids();
     if (tid == 0) {
         prefetch_tensormap(&tmap_q);
         prefetch_tensormap(&tmap_k);
         prefetch_tensormap(&tmap_v);
-        mbar_init(bar_q, 1);
+        for (int i = 0; i < CH_RING; ++i) mbar_init(&bar_u[i], 1);
         for (int s = 0; s < CH_STAGES; ++s) mbar_init(&bar_k[s], 1);
         for (int s = 0; s < CH_VSTAGES; ++s) mbar_init(&bar_v[s], 1);
         for (int s = 0; s < 2; ++s) {
+            mbar_init(&bar_q[s], 1);
             mbar_init(&bar_s[s], 1);
             mbar_init(&bar_o[s], 1);
             mbar_init(&bar_p[s], CH_M / 32);
@@ -277,6 +282,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         tmem_alloc(tmem_slot, CH_TMEM_COLS);
         tmem_relinquish();
     }
+    pdl_wait_prior_grids();  // lengths and tables may come from the grid before
     // ---- lengths: `width` lanes to a row, a run of rows to each such group of lanes ----------------------
     int width = 1;
     while (width < 32 && width < p.n_qtiles) width *= 2;
@@ -351,10 +357,9 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
     before = __shfl_sync(0xffffffffu, before, lane & ~(width - 1));  // of the group's first lane: tiles before its rows
     const bool dealt = chunk_dealt(p, least, most, all, items, longest, (int)gridDim.x);
-    if (dealt) {
-        if (blockIdx.x == 0 && tid == 0 && p.phases) p.plan[1] = 0;
-    } else {
-        // where the phases begin, and the places of all tiles for the kernel behind
+    if (tid < p.phases) p.plan[tid * gridDim.x + blockIdx.x].at = -1;
+    if (!dealt) {
+        // where the phases begin
         if (tid == 0) s_bound[p.phases] = all;
         for (int b = b_lo, base = before; b < b_hi; ++b) {
             const ChunkRow r = chunk_row(p, b);
@@ -363,16 +368,6 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
                 const int pair = f * p.phase_pairs - b * p.Hkv;
                 if (member == 0 && pair >= 0 && pair < p.Hkv) s_bound[f] = base + pair * n;
             }
-            if (b % (int)gridDim.x == (int)blockIdx.x && member == 0) {
-                int32_t *plan = p.plan + CH_PLAN + (long long)b * (p.n_qtiles + 2);
-                plan[0] = base;
-                plan[1] = n;
-                int at = 0;
-                for (int qt = 0; qt * p.tile_tokens < r.n; ++qt) {
-                    plan[2 + qt] = at;
-                    at += chunk_span(p, r, qt * p.tile_tokens).count;
-                }
-            }
             base += n * p.Hkv;
         }
         __syncthreads();
@@ -380,11 +375,6 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             const int lo = s_bound[f], hi = s_bound[f + 1];
             const int each = p.phases == 1 && gridDim.x == 1 ? max(hi - lo, 1) : max((hi - lo + (int)gridDim.x - 1) / (int)gridDim.x, CH_MIN_TILES);
             const int from = (int)min(lo + (long long)each * blockIdx.x, (long long)hi);
-            if (blockIdx.x == 0 && tid == 0) {
-                p.plan[CH_PLAN - 1] = (int)gridDim.x;
-                p.plan[2 * f] = lo;
-                p.plan[2 * f + 1] = each;
-            }
             if (from >= hi) continue;
             for (int b = b_lo, base = before; b < b_hi && base <= from; ++b) {
                 const ChunkRow r = chunk_row(p, b);
@@ -398,12 +388,14 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
                 st.hkv = rel / n;
                 st.off = rel - st.hkv * n;
                 st.qt = 0;
+                int count;
                 for (;; ++st.qt) {
-                    const int count = chunk_span(p, r, st.qt * p.tile_tokens).count;
+                    count = chunk_span(p, r, st.qt * p.tile_tokens).count;
                     if (st.off < count) break;
                     st.off -= count;
                 }
                 s_stretch[f] = st;
+                if (p.phases) p.plan[f * gridDim.x + blockIdx.x] = ChunkPlan{st.at, st.off, count, b, st.hkv, st.qt * p.tile_tokens, lo, each};
             }
         }
     }
@@ -419,74 +411,133 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         atomicOr(p.status, (int)NCKV_ST_TIMEOUT);
     };
     auto par2 = [](uint32_t g) -> uint32_t { return (g >> 1) & 1u; };
+    // Q in one buffer of two halves of 128 rows, or two buffers where a piece has at most 64 rows (the product reads 128 all the same:
+    // what it finds behind them only reaches rows that nobody looks at)
+    const uint32_t q_bufs = p.part_rows <= CH_M / 2 ? 2 : 1, q_half = CH_Q_BYTES / 2 / q_bufs;
 
     if (warp == CH_M / 32 + 1) {
         // =============== one lane moves the tiles ===================================================
         if (elect_one()) {
-            ChunkCursor kc, vc, wc;  // next K tile, next V tile, tile whose score product is awaited
+            ChunkCursor kc;  // next K tile
             kc.start(p, s_stretch, dealt);
-            vc = kc;
-            wc = kc;
-            uint32_t gk = 0, gv = 0, nq = 0;
-            // Boxes outside [kv_lo, kv_hi) need no page: they read as zeros, as pages outside the pool do.
-            auto load_tile = [&](uint8_t *dst, const CUtensorMap *map, uint64_t *bar, const ChunkCursor &c) {
+            uint32_t gk = 0, gv = 0, nu = 0, nq = 0;  // copies issued; pieces posted, their Q tiles asked for
+            auto post = [&](bool more) {
+                ChunkUnit &u = ring[nu % CH_RING];
+                u = kc.u;
+                if (!more) u.n_tiles = 0;
+                mbar_arrive(&bar_u[nu % CH_RING]);
+                ++nu;
+            };
+            // The places of a tile's boxes, looked up a tile ahead of its copies.  Boxes outside [kv_lo, kv_hi) need no page: they read as
+            // zeros, as pages outside the pool do.
+            struct Places {
+                int idx, tok;  // page of the row and token in it at which the next tile begins
+                int page[4], at[4], need;
+            };
+            auto look_up = [&](Places &pl, const ChunkUnit &u, int t) {
+                const int key0 = (u.tile0 + t) * CH_N;
+                if (t == 0) {
+                    pl.idx = key0 / p.page_tokens;
+                    pl.tok = key0 - pl.idx * p.page_tokens;
+                }
+                pl.need = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = key0 + i * p.box;
+                    if (i * p.box >= CH_N) break;
+                    pl.at[i] = pl.tok;
+                    if (key < u.kv_hi && key + p.box > u.kv_lo) {
+                        pl.page[i] = __ldg(p.table + (long long)u.b * p.max_pages + pl.idx);
+                        pl.need |= 1 << i;
+                    }
+                    pl.tok += p.box;
+                    if (pl.tok >= p.page_tokens) {
+                        pl.tok -= p.page_tokens;
+                        ++pl.idx;
+                    }
+                }
+            };
+            auto load_tile = [&](uint8_t *dst, const CUtensorMap *map, uint64_t *bar, const Places &pl, int hkv) {
                 mbar_arrive_expect_tx(bar, CH_KV_BYTES);
-                const int key0 = (c.u.tile0 + c.t) * CH_N;
-                for (int i = 0; i < CH_N; i += p.box) {
-                    const int key = key0 + i, idx = key / p.page_tokens;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (i * p.box >= CH_N) break;
                     int page = p.n_pages;
-                    if (key < c.u.kv_hi && key + p.box > c.u.kv_lo) {
-                        page = __ldg(p.table + (long long)c.u.b * p.max_pages + idx);
+                    if (pl.need >> i & 1) {
+                        page = pl.page[i];
                         if (page < 0 || page >= p.n_pages) {
                             atomicOr(p.status, (int)NCKV_ST_BAD_PAGE);
                             page = p.n_pages;
                         }
                     }
-                    tma_load_4d(dst + i * 128, map, bar, 0, c.u.hkv, key - idx * p.page_tokens, page);
-                    tma_load_4d(dst + CH_KV_BYTES / 2 + i * 128, map, bar, 64, c.u.hkv, key - idx * p.page_tokens, page);
+                    tma_load_4d(dst + i * p.box * 128, map, bar, 0, hkv, pl.at[i], page);
+                    tma_load_4d(dst + CH_KV_BYTES / 2 + i * p.box * 128, map, bar, 64, hkv, pl.at[i], page);
                 }
             };
+            Places kp, vp;
+            uint32_t vu = 0;  // piece and key tile of the next V tile
+            int vt = 0;
+            bool v_known = true;  // its places
             auto load_k = [&]() {
                 const int stage = (int)(gk % CH_STAGES);
-                load_tile(sK + stage * CH_KV_BYTES, &tmap_k, &bar_k[stage], kc);
+                load_tile(sK + stage * CH_KV_BYTES, &tmap_k, &bar_k[stage], kp, kc.u.hkv);
+                const bool ends = kc.last_of_unit();
                 kc.advance(p, s_stretch);
                 ++gk;
+                if (ends) post(kc.valid);
+                if (kc.valid) look_up(kp, kc.u, kc.t);
             };
             auto load_v = [&]() {
                 const int stage = (int)(gv % CH_VSTAGES);
-                load_tile(sV + stage * CH_KV_BYTES, &tmap_v, &bar_v[stage], vc);
-                vc.advance(p, s_stretch);
+                const ChunkUnit &u = ring[vu % CH_RING];
+                if (!v_known) look_up(vp, u, vt);
+                load_tile(sV + stage * CH_KV_BYTES, &tmap_v, &bar_v[stage], vp, u.hkv);
                 ++gv;
+                if (++vt == u.n_tiles) {
+                    vt = 0;
+                    ++vu;
+                }
+                v_known = gv < gk;  // V follows K: its piece is posted
+                if (v_known) look_up(vp, ring[vu % CH_RING], vt);
             };
-            auto load_q = [&](const ChunkUnit &u) {
-                mbar_arrive_expect_tx(bar_q, (uint32_t)(p.tile_tokens * p.G * NCKV_D * 2));
-                tma_load_4d(sQ, &tmap_q, bar_q, 0, u.hkv * p.G, u.t0, u.b);
-                tma_load_4d(sQ + CH_Q_BYTES / 2, &tmap_q, bar_q, 64, u.hkv * p.G, u.t0, u.b);
+            auto load_q = [&]() {
+                const ChunkUnit &u = ring[nq % CH_RING];
+                const uint32_t buf = nq % q_bufs;
+                uint8_t *dst = sQ + buf * (CH_Q_BYTES / 2);
+                mbar_arrive_expect_tx(&bar_q[buf], (uint32_t)(p.tile_tokens * p.G * NCKV_D * 2));
+                tma_load_4d(dst, &tmap_q, &bar_q[buf], 0, u.hkv * p.G, u.t0, u.b);
+                tma_load_4d(dst + q_half, &tmap_q, &bar_q[buf], 64, u.hkv * p.G, u.t0, u.b);
                 ++nq;
             };
             bool ok = true;
-            if (wc.valid) {
-                load_q(wc.u);
+            post(kc.valid);
+            if (kc.valid) {
+                load_q();
+                look_up(kp, kc.u, 0);
+                look_up(vp, kc.u, 0);
+                // V behind K, whose pieces it takes
                 while (gk < CH_STAGES && kc.valid) load_k();
-                while (gv < CH_VSTAGES && vc.valid) load_v();
-                for (uint32_t g = 0; wc.valid && ok; ++g) {
-                    // what S(g)'s completion releases: the Q buffer if g ends its piece, K(g)'s stage for
+                while (gv < CH_VSTAGES && gv < gk) load_v();
+                uint32_t wu = 0;  // piece of the tile whose score product is awaited
+                int left = ring[0].n_tiles;
+                for (uint32_t g = 0;; ++g) {
+                    // Q of a piece ahead where there is room for it
+                    while (nq < wu + q_bufs && nq < nu && ring[nq % CH_RING].n_tiles) load_q();
+                    // what S(g)'s completion releases: a Q buffer if g ends its piece, K(g)'s stage for
                     // K(g+2) and, P V(g-2) being complete too, V(g-2)'s stage for V(g+1)
-                    const bool ends = wc.last_of_unit();
-                    ChunkCursor nx = wc;
-                    nx.advance(p, s_stretch);
-                    if (!kc.valid && !vc.valid && !nx.valid) break;
                     ok = mbar_wait_bounded(&bar_s[g & 1], par2(g));
                     if (!ok) break;
-                    if (ends && nx.valid) load_q(nx.u);
+                    if (--left == 0) {  // the next piece was posted behind the copy of this one's last keys
+                        left = ring[++wu % CH_RING].n_tiles;
+                        if (left == 0) break;
+                    }
                     if (kc.valid) load_k();
-                    if (vc.valid && gv <= g + 1) load_v();
-                    wc = nx;
+                    while (gv < gk && gv <= (g ? g + 1 : CH_VSTAGES - 1)) load_v();
                 }
             }
             if (!ok) timed_out();
             if (*abort_flag) {  // the last copies may still be under way
-                if (nq) mbar_wait_bounded(bar_q, (nq - 1) & 1u);
+                for (uint32_t s = 0; s < q_bufs && s < nq; ++s) mbar_wait_bounded(&bar_q[(nq - 1 - s) % q_bufs], ((nq - 1 - s) / q_bufs) & 1u);
                 for (uint32_t s = 0; s < CH_STAGES && s < gk; ++s) mbar_wait_bounded(&bar_k[(gk - 1 - s) % CH_STAGES], ((gk - 1 - s) / CH_STAGES) & 1u);
                 for (uint32_t s = 0; s < CH_VSTAGES && s < gv; ++s) mbar_wait_bounded(&bar_v[(gv - 1 - s) % CH_VSTAGES], ((gv - 1 - s) / CH_VSTAGES) & 1u);
             }
@@ -498,16 +549,17 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             const uint64_t desc_q = smem_desc_sw128(smem_u32(sQ), 16, 1024);
             const uint64_t desc_k = smem_desc_sw128(smem_u32(sK), 16, 1024);
             const uint64_t desc_v = smem_desc_sw128(smem_u32(sV), CH_KV_BYTES / 2, 1024);
-            ChunkCursor sc, pc;  // tile of the next score product, tile of the next P V product
-            sc.start(p, s_stretch, dealt);
-            pc = sc;
-            uint32_t gs = 0, gp = 0, n_q = 0;
+            uint32_t gs = 0, gp = 0, su = 0, pu = 0;  // tiles and pieces of the next score product and of the next P V product
+            int s_n = 0, s_t = 0, p_t = 0;            // key tiles of the piece; tile inside it
+            auto next_piece = [&]() -> bool {
+                if (!mbar_wait_bounded(&bar_u[su % CH_RING], (su / CH_RING) & 1u)) return false;
+                s_n = ring[su % CH_RING].n_tiles;
+                return true;
+            };
             auto issue_s = [&]() -> bool {
                 const uint32_t stage = gs % CH_STAGES;
-                if (sc.t == 0) {  // first tile of a piece: its Q
-                    if (!mbar_wait_bounded(bar_q, n_q & 1u)) return false;
-                    ++n_q;
-                }
+                const uint32_t buf = su % q_bufs;
+                if (s_t == 0 && !mbar_wait_bounded(&bar_q[buf], (su / q_bufs) & 1u)) return false;  // first tile of a piece: its Q
                 if (!mbar_wait_bounded(&bar_k[stage], (gs / CH_STAGES) & 1u)) return false;
                 tc_fence_after();
                 const uint64_t dk = desc_k + (uint64_t)((stage * CH_KV_BYTES) >> 4);
@@ -515,19 +567,21 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 #pragma unroll
                 for (int kk = 0; kk < NCKV_D / 16; ++kk) {
                     const uint32_t off = (uint32_t)(kk & 3) * 32;
-                    const uint64_t da = desc_q + (uint64_t)(((kk >> 2) * (CH_Q_BYTES / 2) + off) >> 4);
+                    const uint64_t da = desc_q + (uint64_t)((buf * (CH_Q_BYTES / 2) + (kk >> 2) * q_half + off) >> 4);
                     const uint64_t db = dk + (uint64_t)(((kk >> 2) * (CH_KV_BYTES / 2) + off) >> 4);
                     umma_bf16(ds, da, db, IDESC_S, kk > 0 ? 1u : 0u);
                 }
                 umma_commit(&bar_s[gs & 1u]);
-                sc.advance(p, s_stretch);
                 ++gs;
-                return true;
+                if (++s_t < s_n) return true;
+                s_t = 0;
+                ++su;
+                return next_piece();
             };
-            bool ok = true;
-            if (sc.valid) ok = issue_s();
-            if (ok && sc.valid) ok = issue_s();
-            while (pc.valid && ok) {
+            bool ok = next_piece();
+            if (ok && s_n) ok = issue_s();
+            if (ok && s_n) ok = issue_s();
+            while (gp < gs && ok) {
                 // P(gp) is in TMEM, S(gp) has been read, O carries the scale P was made with
                 const uint32_t vstage = gp % CH_VSTAGES;
                 ok = mbar_wait_bounded(&bar_p[gp & 1u], par2(gp)) && mbar_wait_bounded(&bar_v[vstage], (gp / CH_VSTAGES) & 1u);
@@ -538,12 +592,16 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 #pragma unroll
                 for (int ks = 0; ks < CH_N / 16; ++ks) {
                     const uint64_t db = dv + (uint64_t)((ks * 16 * 128) >> 4);
-                    umma_bf16_a_tmem(tmem_o, pbase + (uint32_t)ks * 8, db, IDESC_O, (pc.t > 0 || ks > 0) ? 1u : 0u);
+                    umma_bf16_a_tmem(tmem_o, pbase + (uint32_t)ks * 8, db, IDESC_O, (p_t > 0 || ks > 0) ? 1u : 0u);
                 }
-                const int from_end = pc.u.n_tiles - 1 - pc.t;
+                const int from_end = ring[pu % CH_RING].n_tiles - 1 - p_t;
                 if (from_end < 2) umma_commit(&bar_o[from_end]);
-                if (sc.valid) ok = issue_s();
-                pc.advance(p, s_stretch);
+                if (s_n) ok = issue_s();
+                ++p_t;
+                if (from_end == 0) {
+                    p_t = 0;
+                    ++pu;
+                }
                 ++gp;
             }
             if (!ok) timed_out();
@@ -572,9 +630,13 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             __syncwarp();  // orders the lanes' later reads of the tile behind lane 0's observation
             return ok != 0;
         };
-        ChunkCursor cur;
-        for (cur.start(p, s_stretch, dealt); cur.valid && !aborted; cur.load(p, s_stretch)) {
-            const ChunkUnit &it = cur.u;
+        for (uint32_t seq = 0; !aborted; ++seq) {
+            if (!warp_wait(&bar_u[seq % CH_RING], (seq / CH_RING) & 1u)) {
+                aborted = true;
+                break;
+            }
+            const ChunkUnit it = ring[seq % CH_RING];
+            if (it.n_tiles == 0) break;
             const int n_tiles = it.n_tiles, first_pos = it.L + it.t0, tokens = min(p.tile_tokens, it.n - it.t0);
             const int pos = first_pos + tok;  // absolute position of this row's token
             const bool live = tok < tokens;
@@ -677,7 +739,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
                                 uint16_t *e = reinterpret_cast<uint16_t *>(w);
                                 for (int k = 0; k < 8; ++k)
                                     if ((e[k] & 0x7f80u) == 0x7f80u) e[k] = 0;
-                                s_poison[cur.seq & 3] = cur.seq;
+                                s_poison[seq & 3] = (int)seq;
                             }
                         }
                     }
@@ -697,7 +759,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             }
             tc_fence_after();
             if (warp_live) {
-                const bool poison = s_poison[cur.seq & 3] == cur.seq;
+                const bool poison = s_poison[seq & 3] == (int)seq;
                 const float inv = it.slot >= 0 ? 1.f : (l_run > 0.f ? 1.f / l_run : (l_run == l_run ? 0.f : l_run));
                 const long long part = (long long)it.slot * p.part_rows + row;
                 uint4 *dst = reinterpret_cast<uint4 *>(p.out + (((long long)it.b * p.T + it.t0 + tok) * p.Hq + it.hkv * p.G + head) * NCKV_D);
@@ -747,55 +809,40 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     if (warp == 0) tmem_dealloc(tmem_base, CH_TMEM_COLS);
 }
 
-// Adds up the parts of every query row whose keys were cut: O = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s.  WARPS warps to a row.
+// Adds up the parts of a tile of queries whose keys were cut: O = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s.  Block (CTA, rows, phase) looks at
+// the cut where that CTA's stretch begins and takes the tile's rows if it is the tile's first cut; WARPS warps to a row.
+constexpr int CH_FINISH_ROWS = 4;  // of a warp
 template <int WARPS>
 __global__ void __launch_bounds__(256) chunk_finish_kernel(const __grid_constant__ ChunkParams p) {
     pdl_wait_prior_grids();
-    constexpr int ROWS = 8 / WARPS;
-    __shared__ float4 s_o[8][32];
-    __shared__ float2 s_ml[8];
+    __shared__ float4 s_o[WARPS > 1 ? 8 : 1][32];
+    __shared__ float s_l[8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = warp % WARPS;
-    if (p.plan[1] == 0) return;  // dealt
-    const int grid = p.plan[CH_PLAN - 1];
-    const long long n_rows = (long long)p.B * p.T * p.Hq;
-    for (long long r0 = (long long)blockIdx.x * ROWS; r0 < n_rows; r0 += (long long)gridDim.x * ROWS) {
-        const long long at = r0 + warp / WARPS;
-        // the tile's key tiles begin at `from`; its parts lie in the slots of `count` CTAs from `first` on, whose stretches begin at begin + c each
-        int first = 0, count = 0, from = 0, begin = 0, each = 1, phase = 0, in_unit = 0;
-        if (at < n_rows) {
-            const int hq = (int)(at % p.Hq), t = (int)(at / p.Hq % p.T), b = (int)(at / p.Hq / p.T);
-            const int hkv = hq / p.G, qt = t / p.tile_tokens;
-            const ChunkRow r = chunk_row(p, b);
-            in_unit = (t - qt * p.tile_tokens) * p.G + hq - hkv * p.G;
-            if (t < r.n) {
-                const int32_t *plan = p.plan + CH_PLAN + (long long)b * (p.n_qtiles + 2);
-                const int tiles = chunk_span(p, r, qt * p.tile_tokens).count;
-                phase = (b * p.Hkv + hkv) / p.phase_pairs;
-                begin = p.plan[2 * phase];
-                each = p.plan[2 * phase + 1];
-                from = plan[0] + hkv * plan[1] + plan[2 + qt];
-                first = (from - begin) / each;
-                count = (from - begin + tiles - 1) / each - first + 1;
-                if (count == 1) count = 0;  // written already
-            }
-        }
-        auto part_of = [&](int i) -> long long {  // row of part i
-            const int c = first + i;
-            const long long slot = ((long long)phase * grid + c) * 2 + (begin + c * each < from);  // + 1: not the first piece of the stretch
-            return slot * p.part_rows + in_unit;
-        };
+    const int c = (int)blockIdx.x, grid = (int)gridDim.x, phase = (int)blockIdx.z;
+    const ChunkPlan cut = p.plan[phase * grid + c];
+    if (cut.at < 0 || cut.off == 0) return;
+    const int from = cut.at - cut.off - cut.begin, first = from / cut.each, last = (from + cut.count - 1) / cut.each, parts = last - first + 1;
+    if (c != first + 1) return;
+    const int n = chunk_row(p, cut.b).n, rows = min(p.tile_tokens, n - cut.t0) * p.G;
+    const long long slot0 = ((long long)phase * grid + first) * 2;
+    const bool second = first * cut.each < from;  // the first part is not the first piece of its stretch
+    auto part_of = [&](int i, int row) -> long long { return (slot0 + 2 * i + (i == 0 && second)) * p.part_rows + row; };
+    constexpr int STEP = 8 / WARPS;
+    const int row0 = (int)blockIdx.y * STEP * (WARPS > 1 ? 1 : CH_FINISH_ROWS) + warp / WARPS;
+#pragma unroll 1
+    for (int k = 0; k < (WARPS > 1 ? 1 : CH_FINISH_ROWS); ++k) {
+        const int row = row0 + k * STEP;
+        if (row >= rows) return;  // uniform over the warps of a row
         float m = -INFINITY, l = 0.f;
-        for (int i = lane; i < count; i += 32) {
-            m = fmaxf(m, p.part_ml[part_of(i) * 2]);
-        }
+        for (int i = lane; i < parts; i += 32) m = fmaxf(m, p.part_ml[part_of(i, row) * 2]);
 #pragma unroll
         for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-        for (int i = mine; i < count; i += WARPS) {
-            const long long at_part = part_of(i);
-            const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + at_part * 2);
-            const float4 x = reinterpret_cast<const float4 *>(p.part_o + at_part * NCKV_D)[lane];
+        for (int i = mine; i < parts; i += WARPS) {
+            const long long at = part_of(i, row);
+            const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + at * 2);
+            const float4 x = reinterpret_cast<const float4 *>(p.part_o + at * NCKV_D)[lane];
             if (ml.x == -INFINITY && ml.y == 0.f) continue;  // this row sees none of the part's keys
             const float w = exp2f(ml.x - m);
             l += w * ml.y;
@@ -804,31 +851,33 @@ __global__ void __launch_bounds__(256) chunk_finish_kernel(const __grid_constant
             o.z += w * x.z;
             o.w += w * x.w;
         }
-        if (WARPS > 1) {
+        if constexpr (WARPS > 1) {
             s_o[warp][lane] = o;
-            if (lane == 0) s_ml[warp] = make_float2(m, l);
+            if (lane == 0) s_l[warp] = l;
             __syncthreads();
-            if (mine == 0) {
+            if (mine) return;
 #pragma unroll
-                for (int w = 1; w < WARPS; ++w) {
-                    const float4 x = s_o[warp + w][lane];
-                    l += s_ml[warp + w].y;
-                    o.x += x.x;
-                    o.y += x.y;
-                    o.z += x.z;
-                    o.w += x.w;
-                }
+            for (int w = 1; w < WARPS; ++w) {
+                const float4 x = s_o[warp + w][lane];
+                l += s_l[warp + w];
+                o.x += x.x;
+                o.y += x.y;
+                o.z += x.z;
+                o.w += x.w;
             }
-            __syncthreads();
         }
-        if (mine == 0 && count) {
-            const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-            reinterpret_cast<uint2 *>(p.out + at * NCKV_D)[lane] = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-        }
+        const int tok = row / p.G, head = cut.hkv * p.G + row - tok * p.G;
+        const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+        reinterpret_cast<uint2 *>(p.out + (((long long)cut.b * p.T + cut.t0 + tok) * p.Hq + head) * NCKV_D)[lane] =
+            make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
     }
 }
 
-static size_t chunk_smem_bytes() { return CH_Q_BYTES + (CH_STAGES + CH_VSTAGES) * CH_KV_BYTES + 12 * sizeof(uint64_t) + (2 + 4 + 6 * CH_PHASES + CH_PHASES + 1 + 30) * 4; }
+static size_t chunk_smem_bytes() {
+    return CH_Q_BYTES + (CH_STAGES + CH_VSTAGES) * CH_KV_BYTES + (13 + CH_RING) * sizeof(uint64_t) + CH_RING * sizeof(ChunkUnit) + 6 * 4 +
+           CH_PHASES * sizeof(ChunkStretch) + (CH_PHASES + 1) * 4;
+}
+static_assert(CH_RING * sizeof(ChunkUnit) >= 30 * 4, "the sums over the rows lie where the pieces come later");
 
 // How a launch of these sizes is cut: what of it doesn't depend on the rows' lengths.
 struct ChunkShape {
@@ -858,7 +907,7 @@ static ChunkShape chunk_shape(int B, int T, int Hq, int Hkv, long long capacity,
     s.phase_pairs = (int)((pairs + s.phases - 1) / s.phases);
     s.phases = (int)((pairs + s.phase_pairs - 1) / s.phase_pairs);
     if (s.grid == 1) s.phases = 0;
-    s.plan_bytes = ((size_t)(CH_PLAN + (size_t)B * (s.n_qtiles + 2)) * 4 + 255) / 256 * 256;
+    s.plan_bytes = ((size_t)s.phases * s.grid * sizeof(ChunkPlan) + 255) / 256 * 256;
     return s;
 }
 static size_t chunk_workspace(const ChunkShape &s) {
@@ -943,7 +992,7 @@ extern "C" int nckv_prefill_attn_paged(const void *q, const void *k_pool, const 
     p.new_tokens = new_tokens;
     p.v_pool = static_cast<const __nv_bfloat16 *>(v_pool);
     p.out = static_cast<__nv_bfloat16 *>(out);
-    p.plan = static_cast<int32_t *>(workspace);
+    p.plan = static_cast<ChunkPlan *>(workspace);
     p.part_o = p.part_ml = nullptr;
     if (s.phases) {
         p.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + s.plan_bytes);
@@ -994,10 +1043,10 @@ extern "C" int nckv_prefill_attn_paged(const void *q, const void *k_pool, const 
     cfg.numAttrs = 1;
     NCKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, chunk_attn_kernel, mq, mk, mv, p));
     if (s.phases) {
-        const long long rows = (long long)B * T * Hq, most = 8LL * sm_count();
-        const bool wide = rows <= 2LL * sm_count();
-        const long long blocks = wide ? rows : (rows + 7) / 8;
-        cfg.gridDim = dim3((unsigned)(blocks < most ? blocks : most));
+        // few rows: all of a block's warps to one, over the parts
+        const bool wide = s.part_rows <= 16;
+        const int step = wide ? 1 : 8 * CH_FINISH_ROWS;
+        cfg.gridDim = dim3((unsigned)s.grid, (unsigned)((s.part_rows + step - 1) / step), (unsigned)s.phases);
         cfg.blockDim = dim3(256);
         cfg.dynamicSmemBytes = 0;
         NCKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, wide ? chunk_finish_kernel<8> : chunk_finish_kernel<1>, p));
