@@ -45,6 +45,7 @@ extern "C" {
 #define NCKV_ST_OVERFLOW 1u   /* cache_seqlens[b] + T_new > T_max, or position >= rope_len: row skipped */
 #define NCKV_ST_TIMEOUT 2u    /* a bounded wait on a shared-memory barrier ran out */
 #define NCKV_ST_BAD_SEQLEN 4u /* negative cache_seqlens[b] */
+#define NCKV_ST_BAD_ADAPTER 16u /* an adapter slot outside the bank: the row went without */
 #define NCKV_ST_BAD_PAGE 8u   /* a block-table entry outside the page pool: the tile was read as zeros / the row not written */
 
 /* Library version and the SM architecture the kernels were compiled for ("sm_100a"). */
@@ -569,6 +570,17 @@ NCKV_API int nckv_experts_scratch(const void *a, const void *w, void *out, const
 
 /* out (rows, N) = silu(g) * u with [g; u] = w h, w (2 N, K) gate rows, then up rows, h (rows, K), bf16, K a multiple of 8, fp32 in between. */
 NCKV_API int nckv_gate_up(const void *h, const void *w, void *out, int rows, int N, int K, int32_t *status, void *stream);
+
+/*
+ * Low-rank adapters of B requests beside a projection that they share: row r of request b = r / T with s = slots[b] gets
+ * out_r = bf16(y_r + scales[s] up_s (down_s x_r)), sums in fp32, or out_r = y_r where s < 0 (s >= S: the same, flagged).  bf16 y (B T, N),
+ * x (B T, K) and out (B T, N) with row strides in elements (multiples of 8; out may be y), down (S, R, K) and up (S, N, R) packed; scales
+ * (S) fp32, slots (B) int32.  K, N and R are multiples of 8, R at most 128.  The workspace (16-byte aligned) is the call's own.
+ */
+NCKV_API size_t nckv_adapters_workspace_bytes(int B, int T, int K, int N, int R, int S);
+NCKV_API int nckv_adapters(const void *y, int64_t y_stride, const void *x, int64_t x_stride, const void *down, const void *up,
+                      const int32_t *slots, const float *scales, void *out, int64_t out_stride, int B, int T, int K, int N, int R,
+                      int S, void *workspace, size_t workspace_bytes, int32_t *status, void *stream);
 
 #ifdef __cplusplus
 }

@@ -108,12 +108,15 @@ SIGNATURES = {
     "nckv_route": (c_int, [c_void_p] * 4 + [c_int] * 3 + [c_void_p, c_size_t, c_void_p]),
     "nckv_experts": (c_int, [c_void_p] * 6 + [c_int] * 7 + [c_void_p, c_void_p]),
     "nckv_experts_workspace_bytes": (c_size_t, [c_int] * 6),
+    "nckv_adapters_workspace_bytes": (c_size_t, [c_int] * 6),
+    "nckv_adapters": (c_int, [c_void_p, c_i64, c_void_p, c_i64] + [c_void_p] * 5 + [c_i64] + [c_int] * 6 +
+                      [c_void_p, c_size_t, c_void_p, c_void_p]),
     "nckv_gate_up": (c_int, [c_void_p] * 3 + [c_int] * 3 + [c_void_p] * 2),
     "nckv_experts_scratch": (c_int, [c_void_p] * 6 + [c_int] * 7 + [c_void_p, c_size_t, c_void_p, c_void_p]),
 }
 
 ERROR_NAMES = {-1: "NCKV_E_ARG", -2: "NCKV_E_UNSUPPORTED", -3: "NCKV_E_CAPACITY", -4: "NCKV_E_CUDA"}
-ST_OVERFLOW, ST_TIMEOUT, ST_BAD_SEQLEN, ST_BAD_PAGE = 1, 2, 4, 8
+ST_OVERFLOW, ST_TIMEOUT, ST_BAD_SEQLEN, ST_BAD_PAGE, ST_BAD_ADAPTER = 1, 2, 4, 8, 16
 
 
 class NckvError(RuntimeError):

@@ -119,7 +119,7 @@ def workspace(device, B, Hq, Hkv):
 
 def read_status(device, clear=True):
     """Synchronously read (and by default clear) the device status word of the current stream's
-    workspace (and of the device's latest attention backward); 0 means no guard fired.  Bits: 1 overflow, 2 timeout, 4 bad cache_seqlens, 8 bad page."""
+    workspace (and of the device's latest attention backward); 0 means no guard fired.  Bits: 1 overflow, 2 timeout, 4 bad cache_seqlens, 8 bad page, 16 bad adapter slot."""
     device = torch.device(device)
     idx = device.index if device.index is not None else torch.cuda.current_device()
     key = (idx, torch.cuda.current_stream(idx).cuda_stream)
@@ -141,7 +141,7 @@ def check_status(device):
     st = read_status(device, clear=True)
     if st:
         names = [n for bit, n in ((1, "capacity overflow"), (2, "barrier timeout"), (4, "negative cache_seqlens"),
-                                  (8, "block-table entry outside the page pool")) if st & bit]
+                                  (8, "block-table entry outside the page pool"), (16, "adapter slot outside the bank")) if st & bit]
         raise RuntimeError("nckv device status: " + ", ".join(names))
 
 
@@ -928,6 +928,84 @@ def glue_ve_gate(v, gate_lin, ve):
         _lib.call("nckv_glue_ve_gate", v.data_ptr(), row_stride, gate_lin.data_ptr(), ve.data_ptr(), out.data_ptr(), rows,
                   Hkv, Dh, torch.cuda.current_stream(idx).cuda_stream)
     return out
+
+
+# ------------------------------------------------------------------------------------------------
+# low-rank adapters of many requests
+# ------------------------------------------------------------------------------------------------
+def _activation_rows(t):
+    """Distance between the rows of (..., C) activations, or None where there is no single one of a multiple of 8 elements."""
+    C = t.size(-1)
+    lead = [(n, s) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1]
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(lead[i][1] != lead[i + 1][0] * lead[i + 1][1] for i in range(len(lead) - 1)):
+        return None
+    stride = lead[-1][1] if lead else C
+    return stride if stride >= C and stride % 8 == 0 else None
+
+
+def _adapters(name, y, x, down, up, slots, scales, out):
+    _require_cuda(name, y, x, down, up, slots, scales)
+    _require_bf16(name, y, x, down, up)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (y, x, down, up, scales)):
+        raise RuntimeError(f"nckv::{name} has no backward: call it under torch.no_grad() or inference_mode()")
+    if any(t.device != y.device for t in (x, down, up, slots, scales)):
+        raise RuntimeError(f"nckv::{name}: all tensors must be on {y.device}")
+    if down.dim() != 3 or up.dim() != 3 or y.dim() < 2 or x.shape[:-1] != y.shape[:-1] or x.size(-1) != down.size(2) or \
+            y.size(-1) != up.size(1) or down.size(0) != up.size(0) or down.size(1) != up.size(2):
+        raise RuntimeError(f"nckv::{name}: down {tuple(down.shape)} and up {tuple(up.shape)} do not fit x {tuple(x.shape)} and y {tuple(y.shape)}")
+    if not (down.is_contiguous() and up.is_contiguous()):
+        raise RuntimeError(f"nckv::{name}: down and up must be contiguous")
+    S, R, K = down.shape
+    N, B = up.size(1), slots.numel()
+    if slots.dtype != torch.int32 or slots.dim() != 1 or not slots.is_contiguous() or scales.dtype != torch.float32 or \
+            scales.shape != (S,) or not scales.is_contiguous():
+        raise RuntimeError(f"nckv::{name}: slots must be contiguous int32 of one element per request and scales float32 of {S} elements")
+    rows = y.numel() // N if N else 0
+    if B == 0 or rows % B:
+        if rows == 0 and B == 0:
+            return
+        raise RuntimeError(f"nckv::{name}: {rows} rows do not belong to {B} requests")
+    if rows == 0:
+        return
+    x_stride = _activation_rows(x)
+    if x_stride is None:
+        x = x.contiguous()
+        x = x if x.data_ptr() % 16 == 0 else x.clone()
+        x_stride = K
+    y_stride = _activation_rows(y)
+    if y_stride is None:
+        if out is None:
+            raise RuntimeError(f"nckv::{name}: rows of y {tuple(y.shape)} / {y.stride()} must be packed, 16-byte aligned and one distance apart")
+        y = y.contiguous()
+        y = y if y.data_ptr() % 16 == 0 else y.clone()
+        y_stride = N
+    down, up = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (down, up))
+    out_stride = y_stride if out is None else N
+    status = workspace(y.device, 1, 1, 1)
+    idx = y.device.index
+    with _device_guard(idx):
+        # t = down x between the two launches: the call's own (or the graph's that holds it)
+        need = _lib.lib.nckv_adapters_workspace_bytes(B, rows // B, K, N, R, S)
+        scratch = torch.empty(max(need, 1), dtype=torch.uint8, device=y.device)
+        _lib.call("nckv_adapters", y.data_ptr(), y_stride, x.data_ptr(), x_stride, down.data_ptr(), up.data_ptr(), slots.data_ptr(),
+                  scales.data_ptr(), (y if out is None else out).data_ptr(), out_stride, B, rows // B, K, N, R, S, scratch.data_ptr(), need,
+                  status.data_ptr(), torch.cuda.current_stream(idx).cuda_stream)
+
+
+def add_adapters(y, x, down, up, slots, scales):
+    """y + scales[s] * up[s] (down[s] x) with s = slots[b] for the rows of request b, y where s is negative: what each request's low-rank
+    adapter adds to the output of a projection that all of them share.  x (..., K) and y (..., N) bf16 hold the rows of ``slots.numel()``
+    requests one after the other, as many for each; down (S, R, K), up (S, N, R) bf16; scales (S,) float32; slots int32.  K, N and R are
+    multiples of 8, R at most 128.  Sums in float32, rounded once."""
+    out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    _adapters("add_adapters", y, x, down, up, slots, scales, out)
+    return out
+
+
+def add_adapters_(y, x, down, up, slots, scales):
+    """The same into y, which may be a column slice of a wider product; rows without an adapter are not touched.  Returns y."""
+    _adapters("add_adapters_", y, x, down, up, slots, scales, None)
+    return y
 
 
 class HostDecodeStep:
