@@ -34,11 +34,13 @@ class KVCache:
         self.v_cache = torch.zeros(shape, device=device, dtype=dtype)
         self.cache_seqlens = torch.zeros(batch_size, dtype=torch.int32, device=device)
         self.prev_embedding = None  # smear state owned by the model's forward pass
+        self.adapter_slots = None   # int32 per row: slot in the model's adapter bank, or negative
 
     def reset(self):
         """Empty the cache (engine.py:106-109); storage is kept."""
         self.cache_seqlens.zero_()
         self.prev_embedding = None
+        self.adapter_slots = None
 
     def get_pos(self):
         """Length of row 0 as a Python int (engine.py:111-113). This synchronises with the device;
@@ -80,6 +82,14 @@ class KVCache:
             ops.prefill_broadcast(other.k_cache, other.v_cache, self.k_cache, self.v_cache, self.cache_seqlens, other_pos)
         if other.prev_embedding is not None:
             self.prev_embedding = other.prev_embedding.expand(self.batch_size, -1, -1).clone()
+        _broadcast_adapter(self, other)
+
+
+def _broadcast_adapter(cache, prompt):
+    """A prompt's adapter stays with the rows that continue it."""
+    slots = getattr(prompt, "adapter_slots", None)
+    if slots is not None:
+        cache.adapter_slots = slots.expand(cache.batch_size).clone()
 
 
 class PagedKVCache:
@@ -125,6 +135,7 @@ class PagedKVCache:
         self._count = [0] * batch_size   # pages in each row's table, shared ones included
         self._shared = 0                 # leading pages of every row that all rows share
         self.prev_embedding = None
+        self.adapter_slots = None        # as KVCache's
 
     # ---- the reference's KVCache methods -------------------------------------------------------
     def reset(self):
@@ -135,6 +146,7 @@ class PagedKVCache:
         self.block_table.fill_(-1)
         self.cache_seqlens.zero_()
         self.prev_embedding = None
+        self.adapter_slots = None
 
     def get_pos(self):
         return int(self.cache_seqlens[0].item())
@@ -208,6 +220,7 @@ class PagedKVCache:
         self.cache_seqlens.fill_(p)
         if other.prev_embedding is not None:
             self.prev_embedding = other.prev_embedding.expand(B, -1, -1).clone()
+        _broadcast_adapter(self, other)
 
 
 class HybridCache:
@@ -418,9 +431,13 @@ class Engine:
         self.cuda_graph = cuda_graph
 
     @torch.inference_mode()
-    def generate(self, tokens, num_samples=1, max_tokens=None, temperature=1.0, top_k=None, seed=42):
+    def generate(self, tokens, num_samples=1, max_tokens=None, temperature=1.0, top_k=None, seed=42, adapter=None):
+        """``adapter``: slot of the model's adapter bank that the prompt and its samples run with."""
         assert isinstance(tokens, list) and isinstance(tokens[0], int), "expecting list of ints"
         device = self.model.get_device()
+        bank = getattr(self.model, "adapters", None)
+        if adapter is not None and (bank is None or not 0 <= adapter < bank.slots):
+            raise ValueError(f"the model has no adapter {adapter}")
         dtype = torch.bfloat16 if device.type == "cuda" else torch.float32
         rng = torch.Generator(device=device)
         rng.manual_seed(seed)
@@ -432,6 +449,8 @@ class Engine:
 
         cfg = self.model.config
         prompt_cache = new_cache(self.model, 1, len(tokens), dtype)
+        if adapter is not None:
+            prompt_cache.adapter_slots = torch.tensor([adapter], dtype=torch.int32, device=device)
         ids = torch.tensor([tokens], dtype=torch.long, device=device)
         logits = forward_at(self.model, ids, prompt_cache, [len(tokens) - 1])[:, -1, :].expand(num_samples, -1)
 

@@ -125,6 +125,11 @@ def layer_has_value_embedding(layer_idx, n_layer):
     return layer_idx % 2 == (n_layer - 1) % 2
 
 
+def _alone(name, y, x):
+    """A projection's product without an adapter."""
+    return y
+
+
 class CastLinear(nn.Linear):
     """Bias-free linear whose weight is used in the activation's dtype (gpt.py:45-50).  The cast is
     skipped when the dtypes already agree, e.g. after ``model.to(torch.bfloat16)``."""
@@ -176,11 +181,11 @@ class Attention(nn.Module):
             self._qkv_cache = (key, stacked if same else None)
         return self._qkv_cache[1]
 
-    def forward(self, x, ve, rope_tables, window_size, kv_cache):
+    def forward(self, x, ve, rope_tables, window_size, kv_cache, adapted=_alone):
         B, T, _ = x.shape
-        q = self.c_q(x).view(B, T, self.n_head, self.head_dim)
-        k = self.c_k(x).view(B, T, self.n_kv_head, self.head_dim)
-        v = self.c_v(x).view(B, T, self.n_kv_head, self.head_dim)
+        q = adapted("attn.c_q", self.c_q(x), x).view(B, T, self.n_head, self.head_dim)
+        k = adapted("attn.c_k", self.c_k(x), x).view(B, T, self.n_kv_head, self.head_dim)
+        v = adapted("attn.c_v", self.c_v(x), x).view(B, T, self.n_kv_head, self.head_dim)
         if ve is not None:  # value residual with an input-dependent per-head gate (gpt.py:92-95)
             gate = 3 * torch.sigmoid(self.ve_gate(x[..., :self.ve_gate_channels]))
             v = v + gate.unsqueeze(-1) * ve.view(B, T, self.n_kv_head, self.head_dim)
@@ -192,7 +197,8 @@ class Attention(nn.Module):
             cos, sin = rope_tables[0][:, :T], rope_tables[1][:, :T]
             q, k = _rope_norm_scale(q, cos, sin), _rope_norm_scale(k, cos, sin)
             y = flash_attn.flash_attn_func(q, k, v, causal=True, window_size=window_size)
-        return self.c_proj(y.contiguous().view(B, T, -1))
+        y = y.contiguous().view(B, T, -1)
+        return adapted("attn.c_proj", self.c_proj(y), y)
 
 
 def _rope_norm_scale(x, cos, sin):
@@ -208,8 +214,9 @@ class MLP(nn.Module):
         self.c_fc = CastLinear(config.n_embd, 4 * config.n_embd, bias=False)
         self.c_proj = CastLinear(4 * config.n_embd, config.n_embd, bias=False)
 
-    def forward(self, x):
-        return self.c_proj(F.relu(self.c_fc(x)).square())
+    def forward(self, x, adapted=_alone):
+        h = F.relu(adapted("mlp.c_fc", self.c_fc(x), x)).square()
+        return adapted("mlp.c_proj", self.c_proj(h), h)
 
 
 class Block(nn.Module):
@@ -218,9 +225,10 @@ class Block(nn.Module):
         self.attn = Attention(config, layer_idx)
         self.mlp = MLP(config)
 
-    def forward(self, x, ve, rope_tables, window_size, kv_cache):
-        x = x + self.attn(rms(x), ve, rope_tables, window_size, kv_cache)
-        return x + self.mlp(rms(x))
+    def forward(self, x, ve, rope_tables, window_size, kv_cache, adapted=None):
+        more = {} if adapted is None else {"adapted": adapted}
+        x = x + self.attn(rms(x), ve, rope_tables, window_size, kv_cache, **more)
+        return x + self.mlp(rms(x), **more)
 
 
 _FORWARD = {cls: cls.forward for cls in (CastLinear, Attention, MLP, Block)}
@@ -260,6 +268,7 @@ class GPT(nn.Module):
         # run the eager op sequence everywhere.
         self.fused_glue = True
         self.fused_qkv = True   # one [c_q; c_k; c_v] product per layer in the decode trunk where it is bit-identical
+        self.adapters = None    # an adapters.AdapterBank puts itself here
         self._lambda_cache = None  # stays empty: the scalars are read where they lie, in every pass
         self.rotary_seq_len = config.sequence_len * 10  # same over-allocation as gpt.py:195
         self.register_buffer("cos", torch.empty(0), persistent=False)
@@ -356,13 +365,19 @@ class GPT(nn.Module):
         backout_at = self.config.n_layer // 2
         x_backout = None
         rope_tables = (self.cos, self.sin)
+        slots = getattr(kv_cache, "adapter_slots", None)
+        if slots is not None and self.adapters is None:
+            raise ValueError("the cache's rows name adapters, the model has no bank of them")
+        if slots is not None and slots.shape != (B,):
+            raise ValueError(f"adapter_slots must name one slot for each of {B} rows, got {tuple(slots.shape)}")
         if self.fused_glue and kv_cache is not None and x.is_cuda and x.dtype == torch.bfloat16 and \
                 (T == 1 or self._prompt_can_fuse(B, x.device)):
-            return self._head(self._trunk_fused(idx, x, kv_cache, rope_tables), logits_at)
+            return self._head(self._trunk_fused(idx, x, kv_cache, rope_tables, slots), logits_at)
         for i, block in enumerate(self.transformer.h):
             x = self.resid_lambdas[i] * x + self.x0_lambdas[i] * x0
             ve = self.value_embeds[str(i)](idx).to(x.dtype) if str(i) in self.value_embeds else None
-            x = block(x, ve, rope_tables, self.window_sizes[i], kv_cache)
+            more = {} if slots is None else {"adapted": self.adapters.at(i, slots)}
+            x = block(x, ve, rope_tables, self.window_sizes[i], kv_cache, **more)
             if i == backout_at:
                 x_backout = x
         if x_backout is not None:
@@ -422,7 +437,7 @@ class GPT(nn.Module):
         r, x, b = (t.detach().to(torch.bfloat16).float().reshape(-1).tolist() for t in params)
         return ops.glue_mix_norm, lambda i: dict(resid_lambda=r[i], x0_lambda=x[i]), dict(backout_lambda=b[0])
 
-    def _trunk_fused(self, idx, x, kv_cache, rope_tables):
+    def _trunk_fused(self, idx, x, kv_cache, rope_tables, slots=None):
         """The layer loop of ``forward`` over a cache with the elementwise glue fused, up to the last norm:
         per layer one launch for [previous MLP residual add + lambda mix + norm], one for [attention
         residual add + norm], one for relu^2 (and one for the value-embedding gate where a layer has
@@ -443,24 +458,27 @@ class GPT(nn.Module):
                 x_backout = x_sum
             attn, mlp = block._modules["attn"], block._modules["mlp"]._modules  # (past Module.__getattr__, ten times a layer)
             products = attn._modules
+            adapted = _alone if slots is None else self.adapters.at(i, slots)
             # one token per row: the row count stays, and with it the check; prompts come in all lengths
             w_qkv = attn.fused_qkv_weight(xn) if self.fused_qkv and T == 1 else None
             if w_qkv is not None:  # one product; q, k, v are column slices of its output (the kernels take the stride)
                 nq, nkv = attn.n_head * attn.head_dim, attn.n_kv_head * attn.head_dim
                 qkv = F.linear(xn, w_qkv)
-                q = qkv[..., :nq].view(B, 1, attn.n_head, attn.head_dim)
-                k = qkv[..., nq:nq + nkv].view(B, 1, attn.n_kv_head, attn.head_dim)
-                v = qkv[..., nq + nkv:].view(B, 1, attn.n_kv_head, attn.head_dim)
+                q = adapted("attn.c_q", qkv[..., :nq], xn).view(B, 1, attn.n_head, attn.head_dim)
+                k = adapted("attn.c_k", qkv[..., nq:nq + nkv], xn).view(B, 1, attn.n_kv_head, attn.head_dim)
+                v = adapted("attn.c_v", qkv[..., nq + nkv:], xn).view(B, 1, attn.n_kv_head, attn.head_dim)
             else:
-                q = products["c_q"](xn).view(B, T, attn.n_head, attn.head_dim)
-                k = products["c_k"](xn).view(B, T, attn.n_kv_head, attn.head_dim)
-                v = products["c_v"](xn).view(B, T, attn.n_kv_head, attn.head_dim)
+                q = adapted("attn.c_q", products["c_q"](xn), xn).view(B, T, attn.n_head, attn.head_dim)
+                k = adapted("attn.c_k", products["c_k"](xn), xn).view(B, T, attn.n_kv_head, attn.head_dim)
+                v = adapted("attn.c_v", products["c_v"](xn), xn).view(B, T, attn.n_kv_head, attn.head_dim)
             if str(i) in self.value_embeds:
                 ve = self.value_embeds[str(i)](idx).to(x.dtype)
                 v = ops.glue_ve_gate(v, products["ve_gate"](xn[..., :attn.ve_gate_channels]), ve)
             y = kv_attention(q, k, v, rope_tables, self.window_sizes[i], kv_cache, i)
-            _, x, xn = ops.glue_mix_norm(x, add=products["c_proj"](y.view(B, T, C)))
-            pending = mlp["c_proj"](ops.glue_relu_sq(mlp["c_fc"](xn)))
+            y = y.view(B, T, C)
+            _, x, xn = ops.glue_mix_norm(x, add=adapted("attn.c_proj", products["c_proj"](y), y))
+            h = ops.glue_relu_sq(adapted("mlp.c_fc", mlp["c_fc"](xn), xn))
+            pending = adapted("mlp.c_proj", mlp["c_proj"](h), h)
         if backout_at == n_layer - 1:  # only a one-layer model: the backout operand is the final sum itself
             x_backout, _, _ = ops.glue_mix_norm(x, add=pending, want_sum=True, want_x=False, want_norm=False)
             _, _, xn = mix(x_backout, x_backout=x_backout, want_x=False, **backout)
