@@ -8,28 +8,20 @@
 // the slots: it is for request b and does the work if b is the first of a unit.  mma.sync, operands straight from global memory in
 // 16-byte loads: the order of the channels inside a product is free, so a lane's 8 consecutive ones stand for the two pairs that
 // the instruction wants from it, twice.
-#include "nckv_common.cuh"
+#include "adapters.cuh"
 
 namespace nckv {
 
-constexpr int AD_THREADS = 256, AD_ROWS = 16, AD_MAX_RANK = 128;
+constexpr int AD_THREADS = 256, AD_ROWS = 16;
 
-struct AdapterParams {
-    const __nv_bfloat16 *y, *x, *down, *up;
-    __nv_bfloat16 *out;
-    const int32_t *slots;
-    const float *scales;
-    float *t;  // (splits, rows, R)
-    int32_t *status;
-    long long y_stride, x_stride, out_stride;
-    int B, T, K, N, R, S;
+struct AdapterRows : AdapterParams {
     int chunks;       // units of AD_ROWS tokens per request
     int per_unit;     // requests of one slot that share a unit (1 where a request has several units)
     int splits, k_each, n_each;  // parts of the channels and outputs of a CTA
 };
 
 // Rows of a unit: row numbers in s_row (-1: none), and its slot.  False: nothing to do here.
-__device__ __forceinline__ bool adapter_unit(const AdapterParams &p, int unit, int *s_row, int &slot, int &rows) {
+__device__ __forceinline__ bool adapter_unit(const AdapterRows &p, int unit, int *s_row, int &slot, int &rows) {
     __shared__ int s_before, s_warp[AD_THREADS / 32];
     const int b = unit / p.chunks, chunk = unit - b * p.chunks, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     slot = p.slots[b];
@@ -75,7 +67,7 @@ __device__ __forceinline__ bool adapter_unit(const AdapterParams &p, int unit, i
 
 // t[part][row] = down x over a part of the channels: a warp takes every eighth step of 32 channels, the warps' sums meet in shared memory.
 template <int TILES>  // of 8 ranks
-__global__ void __launch_bounds__(AD_THREADS) adapter_down_kernel(const __grid_constant__ AdapterParams p) {
+__global__ void __launch_bounds__(AD_THREADS) adapter_down_kernel(const __grid_constant__ AdapterRows p) {
     __shared__ int s_row[AD_ROWS];
     __shared__ float s_t[AD_ROWS][TILES * 8 + 1];
     pdl_wait_prior_grids();
@@ -123,7 +115,7 @@ __global__ void __launch_bounds__(AD_THREADS) adapter_down_kernel(const __grid_c
         }
         __syncthreads();
     }
-    float *t = p.t + (long long)blockIdx.y * p.B * p.T * p.R;
+    float *t = static_cast<float *>(p.t) + (long long)blockIdx.y * p.B * p.T * p.R;
     for (int i = threadIdx.x; i < rows * p.R; i += AD_THREADS) {
         const int row = i / p.R, r = i - row * p.R;
         t[(long long)s_row[row] * p.R + r] = s_t[row][r];
@@ -136,7 +128,7 @@ __device__ __forceinline__ float adapter_rest(float t, float hi) { return fabsf(
 // out = y + scale up t over a part of the outputs: a warp takes 32 outputs at a time.  Output column of (product j, column c) is
 // c / 2 * 8 + j * 2 + c % 2 of the 32, so that a lane holds 8 consecutive ones of a row.
 template <int STEPS>  // of 16 ranks
-__global__ void __launch_bounds__(AD_THREADS) adapter_up_kernel(const __grid_constant__ AdapterParams p) {
+__global__ void __launch_bounds__(AD_THREADS) adapter_up_kernel(const __grid_constant__ AdapterRows p) {
     __shared__ int s_row[AD_ROWS];
     pdl_launch_dependents();
     int slot, rows;
@@ -157,6 +149,7 @@ __global__ void __launch_bounds__(AD_THREADS) adapter_up_kernel(const __grid_con
     const float scale = p.scales[slot];
     // t of the two rows, summed over the parts of the channels, as two bf16 terms
     uint32_t hi[STEPS][4], lo[STEPS][4];
+    const float *t = static_cast<const float *>(p.t);
     const long long part = (long long)p.B * p.T * p.R;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
@@ -165,11 +158,11 @@ __global__ void __launch_bounds__(AD_THREADS) adapter_up_kernel(const __grid_con
         if (r < p.R)
             for (int s = 0; s < p.splits; ++s) {
                 if (r0 >= 0) {
-                    const float4 v = *reinterpret_cast<const float4 *>(p.t + s * part + (long long)r0 * p.R + r);
+                    const float4 v = *reinterpret_cast<const float4 *>(t + s * part + (long long)r0 * p.R + r);
                     t0.x += v.x; t0.y += v.y; t0.z += v.z; t0.w += v.w;
                 }
                 if (r1 >= 0) {
-                    const float4 v = *reinterpret_cast<const float4 *>(p.t + s * part + (long long)r1 * p.R + r);
+                    const float4 v = *reinterpret_cast<const float4 *>(t + s * part + (long long)r1 * p.R + r);
                     t1.x += v.x; t1.y += v.y; t1.z += v.z; t1.w += v.w;
                 }
             }
@@ -246,6 +239,7 @@ static int adapter_check_sizes(const char *name, int B, int T, int K, int N, int
 extern "C" size_t nckv_adapters_workspace_bytes(int B, int T, int K, int N, int R, int S) {
     using namespace nckv;
     if (adapter_check_sizes("adapters_workspace_bytes", B, T, K, N, R, S) != NCKV_OK) return 0;
+    if (adapters_tiled(T)) return adapters_tc_bytes(B, T, R);
     const long long units = (long long)B * ((T + AD_ROWS - 1) / AD_ROWS);
     return (size_t)adapter_splits(units, K) * B * T * R * 4;
 }
@@ -273,7 +267,7 @@ extern "C" int nckv_adapters(const void *y, int64_t y_stride, const void *x, int
         set_error("%s: needs %zu bytes of workspace", name, nckv_adapters_workspace_bytes(B, T, K, N, R, S));
         return NCKV_E_CAPACITY;
     }
-    AdapterParams p;
+    AdapterRows p;
     p.y = static_cast<const __nv_bfloat16 *>(y);
     p.x = static_cast<const __nv_bfloat16 *>(x);
     p.down = static_cast<const __nv_bfloat16 *>(down);
@@ -281,10 +275,11 @@ extern "C" int nckv_adapters(const void *y, int64_t y_stride, const void *x, int
     p.out = static_cast<__nv_bfloat16 *>(out);
     p.slots = slots;
     p.scales = scales;
-    p.t = static_cast<float *>(workspace);
+    p.t = workspace;
     p.status = status;
     p.y_stride = y_stride; p.x_stride = x_stride; p.out_stride = out_stride;
     p.B = B; p.T = T; p.K = K; p.N = N; p.R = R; p.S = S;
+    if (adapters_tiled(T)) return adapters_tc(p, static_cast<cudaStream_t>(stream));
     p.chunks = (T + AD_ROWS - 1) / AD_ROWS;
     p.per_unit = T < AD_ROWS ? AD_ROWS / T : 1;
     const long long units = (long long)B * p.chunks;

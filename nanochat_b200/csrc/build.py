@@ -21,8 +21,8 @@ BINDING = os.path.join(HERE, "binding.cpp")
 SOURCES = ["host.cu", "append.cu", "decode_attn.cu", "decode_small.cu", "prefill_broadcast.cu", "lse_combine.cu",
            "prefill_attn.cu", "chunk_attn.cu", "p2p_exchange.cu", "glue.cu", "flash_attn_bwd.cu", "host_step.cu",
            "recurrent.cu", "recurrent_f32.cu", "norm_mix.cu", "window_attn.cu", "hyper_norm.cu",
-           "gated_linear.cu", "delta.cu", "delta_chunk.cu", "experts.cu", "experts_tc.cu", "experts_pair.cu", "linear_cap.cu", "adapters.cu"]
-HEADERS = ["nckv_common.cuh", "vec_io.cuh", "tc05.cuh", "rope_row.cuh", "recurrent.cuh", "experts.cuh", os.path.join("..", "..", "include", "nckv.h")]
+           "gated_linear.cu", "delta.cu", "delta_chunk.cu", "experts.cu", "experts_tc.cu", "experts_pair.cu", "linear_cap.cu", "adapters.cu", "adapters_tc.cu"]
+HEADERS = ["nckv_common.cuh", "vec_io.cuh", "tc05.cuh", "rope_row.cuh", "recurrent.cuh", "experts.cuh", "adapters.cuh", os.path.join("..", "..", "include", "nckv.h")]
 
 
 def _nvcc():
