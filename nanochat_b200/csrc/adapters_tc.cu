@@ -17,7 +17,9 @@
 namespace nckv {
 
 constexpr int AT_M = 128, AT_K = 64, AT_N = 64;
-constexpr int AT_THREADS = 192;  // copies, products, four warps for the accumulator's rows
+constexpr int AT_THREADS = 192;             // copies, products, four warps for the accumulator's rows
+constexpr int AT_UP_THREADS = 64 + 2 * 128;  // two groups of four take steps in turn
+constexpr int AT_ACCS = 4;                   // accumulators of adapter_tile_up
 constexpr int AT_X_BYTES = AT_M * AT_K * 2;
 constexpr int AT_DOWN_STAGES = 4, AT_MAX_CLUSTER = 8;
 
@@ -54,7 +56,6 @@ adapter_tile_down(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     extern __shared__ __align__(1024) uint8_t smem[];
     const AdapterParams &p = q.a;
     pdl_wait_prior_grids();
-    pdl_launch_dependents();  // behind the wait: the next grid reads slots, y and weights ahead of its own
     const int ctas = (int)cluster_ctas(), rank = (int)cluster_rank(), tile = (int)blockIdx.x / ctas;
     const int b = tile / q.tiles, t0 = (tile - b * q.tiles) * AT_M, slot = adapter_slot(p, b);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -85,6 +86,9 @@ adapter_tile_down(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    // Behind the wait: the next grid reads slots, y and weights ahead of its own.  Behind the allocation: its CTAs hold tensor memory while
+    // they wait for this grid.
+    pdl_launch_dependents();
     const uint32_t tmem = *tmem_slot;
     auto timed_out = [&]() {
         *abort_flag = 1;
@@ -188,7 +192,7 @@ adapter_tile_down(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     if (warp == 0) tmem_dealloc(tmem, columns);
 }
 
-__global__ void __launch_bounds__(AT_THREADS, 1)
+__global__ void __launch_bounds__(AT_UP_THREADS, 1)
 adapter_tile_up(const __grid_constant__ CUtensorMap map_t, const __grid_constant__ CUtensorMap map_up, const __grid_constant__ CUtensorMap map_y,
                 const __grid_constant__ CUtensorMap map_out, const __grid_constant__ AdapterTile q) {
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -198,12 +202,12 @@ adapter_tile_up(const __grid_constant__ CUtensorMap map_t, const __grid_constant
     uint8_t *s_t = smem, *ring = smem + t_bytes;
     uint64_t *bars = reinterpret_cast<uint64_t *>(ring + q.stages * stage_bytes);
     uint64_t *bar_full = bars, *bar_free = bars + q.stages;
-    uint64_t *bar_acc = bars + 2 * q.stages, *bar_read = bar_acc + 2, *bar_t = bar_acc + 4, *bar_t_read = bar_acc + 5;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar_acc + 6);
+    uint64_t *bar_acc = bars + 2 * q.stages, *bar_read = bar_acc + AT_ACCS, *bar_t = bar_acc + 2 * AT_ACCS, *bar_t_read = bar_t + 1;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar_t + 2);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (warp == 0) {
-        tmem_alloc(tmem_slot, 2 * AT_N);
+        tmem_alloc(tmem_slot, AT_ACCS * AT_N);
         tmem_relinquish();
     } else if (tid == 32) {
         prefetch_tensormap(&map_t);
@@ -214,7 +218,7 @@ adapter_tile_up(const __grid_constant__ CUtensorMap map_t, const __grid_constant
             mbar_init(&bar_full[i], 1);
             mbar_init(&bar_free[i], 4);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < AT_ACCS; ++i) {
             mbar_init(&bar_acc[i], 1);
             mbar_init(&bar_read[i], 4);
         }
@@ -263,8 +267,8 @@ adapter_tile_up(const __grid_constant__ CUtensorMap map_t, const __grid_constant
                     tma_load_3d(at, &map_y, &bar_full[s], n0, t0, b);
                     if (slot >= 0)
                         for (int k = 0; k < up_boxes; ++k) tma_load_3d(at + y_bytes + k * AT_N * 128, &map_up, &bar_full[s], k * 64, n0, slot);
-                    // t behind as much of the ring as there is room for
-                    if (slot >= 0 && i == min(n, q.stages - 1) - 1) {
+                    // t behind as much of the ring as doesn't need this tile's steps done (a stage is free two steps behind its own)
+                    if (slot >= 0 && i == min(n, q.stages - 2) - 1) {
                         if (!waited) pdl_wait_prior_grids();
                         waited = true;
                         if (n_t) ok = mbar_wait_bounded(bar_t_read, (n_t + 1) & 1);
@@ -299,16 +303,16 @@ adapter_tile_up(const __grid_constant__ CUtensorMap map_t, const __grid_constant
                 ok = mbar_wait_bounded(bar_t, n_t & 1);
                 for (int i = 0; i < n && ok; ++i, ++g, ++m) {
                     const uint32_t s = g % q.stages;
-                    ok = mbar_wait_bounded(&bar_full[s], (g / q.stages) & 1) && (m < 2 || mbar_wait_bounded(&bar_read[m & 1], (m / 2 + 1) & 1));
+                    ok = mbar_wait_bounded(&bar_full[s], (g / q.stages) & 1) && (m < AT_ACCS || mbar_wait_bounded(&bar_read[m % AT_ACCS], (m / AT_ACCS + 1) & 1));
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t desc_up = smem_desc_sw128(smem_u32(ring + s * stage_bytes + y_bytes), 16, 1024);
                     for (int k = 0; k < q.RP / 8; ++k) {  // hi, then lo
                         const int rank = k * 16 % q.RP, col = k * 16;
-                        umma_bf16(tmem + (m & 1) * AT_N, desc_t + (uint64_t)((col / 64 * AT_M * 128 + col % 64 * 2) >> 4),
+                        umma_bf16(tmem + (m % AT_ACCS) * AT_N, desc_t + (uint64_t)((col / 64 * AT_M * 128 + col % 64 * 2) >> 4),
                                   desc_up + (uint64_t)((rank / 64 * AT_N * 128 + rank % 64 * 2) >> 4), IDESC, k > 0);
                     }
-                    umma_commit(&bar_acc[m & 1]);
+                    umma_commit(&bar_acc[m % AT_ACCS]);
                 }
                 if (ok) umma_commit(bar_t_read);
                 ++n_t;
@@ -319,7 +323,7 @@ adapter_tile_up(const __grid_constant__ CUtensorMap map_t, const __grid_constant
         __syncwarp();
     } else {
         // =============== rows: y in the ring becomes the result ==============================================
-        const int part = warp & 3, row = part * 32 + lane;
+        const int part = warp & 3, row = part * 32 + lane, group = (warp - 2) / 4;
         auto warp_wait = [&](uint64_t *bar, uint32_t parity) -> bool {
             if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
             int ok = *abort_flag == 0;
@@ -329,24 +333,25 @@ adapter_tile_up(const __grid_constant__ CUtensorMap map_t, const __grid_constant
             return ok != 0;
         };
         uint32_t g = 0, m = 0;
+        int last = -1;  // stage of this warp's store before
         bool ok = true;
         for_tiles([&](int from, int n, int b, int t0, int slot) {
             const float scale = slot >= 0 ? p.scales[slot] : 0.f;
-            for (int i = 0; i < n; ++i, ++g) {
+            for (int i = 0; i < n; ++i, ++g, m += slot >= 0) {
+                if ((int)(g & 1) != group) continue;
                 const uint32_t s = g % q.stages;
                 uint8_t *y = ring + s * stage_bytes;
                 ok = warp_wait(&bar_full[s], (g / q.stages) & 1);
                 if (!ok) return false;
                 if (slot >= 0) {
-                    ok = warp_wait(&bar_acc[m & 1], (m / 2) & 1);
+                    ok = warp_wait(&bar_acc[m % AT_ACCS], (m / AT_ACCS) & 1);
                     if (!ok) return false;
                     tc_fence_after();
                     float d[AT_N];
-                    tmem_ld64(tmem + (m & 1) * AT_N + ((uint32_t)(part * 32) << 16), d);
+                    tmem_ld64(tmem + (m % AT_ACCS) * AT_N + ((uint32_t)(part * 32) << 16), d);
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&bar_read[m & 1]);
-                    ++m;
+                    if (lane == 0) mbar_arrive(&bar_read[m % AT_ACCS]);
 #pragma unroll
                     for (int c = 0; c < 8; ++c) {
                         uint4 *at = reinterpret_cast<uint4 *>(y + row * 128 + ((c ^ (row & 7)) << 4));
@@ -363,10 +368,11 @@ adapter_tile_up(const __grid_constant__ CUtensorMap map_t, const __grid_constant
                 if (lane == 0) {
                     if (t0 + part * 32 < p.T) tma_store_3d(&map_out, y + part * 32 * 128, (from + i) * AT_N, t0 + part * 32, b);
                     else asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                    if (g) {  // the store before has read its stage
+                    if (last >= 0) {  // the store before has read its stage
                         tma_stores_read<1>();
-                        mbar_arrive(&bar_free[(g - 1) % q.stages]);
+                        mbar_arrive(&bar_free[last]);
                     }
+                    last = (int)s;
                 }
             }
             return true;
@@ -377,7 +383,7 @@ adapter_tile_up(const __grid_constant__ CUtensorMap map_t, const __grid_constant
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) tmem_dealloc(tmem, 2 * AT_N);
+    if (warp == 0) tmem_dealloc(tmem, AT_ACCS * AT_N);
 }
 
 static int rank_pad(int R) { return (R + 15) / 16 * 16; }
@@ -385,7 +391,7 @@ size_t adapters_tc_bytes(int B, int T, int R) { return (size_t)B * T * 2 * rank_
 
 static size_t adapter_down_smem(int RP) { return AT_DOWN_STAGES * (size_t)(AT_X_BYTES + RP * AT_K * 2) + (2 * AT_DOWN_STAGES + 1) * 8 + 16; }
 static size_t adapter_up_smem(int RP, int R, int stages) {
-    return (size_t)(2 * RP + 63) / 64 * AT_M * 128 + (size_t)stages * (AT_M * 128 + (R + 63) / 64 * AT_N * 128) + (2 * stages + 6) * 8 + 16;
+    return (size_t)(2 * RP + 63) / 64 * AT_M * 128 + (size_t)stages * (AT_M * 128 + (R + 63) / 64 * AT_N * 128) + (2 * stages + 2 * AT_ACCS + 2) * 8 + 16;
 }
 
 int adapters_tc(const AdapterParams &a, cudaStream_t stream) {
@@ -416,7 +422,7 @@ int adapters_tc(const AdapterParams &a, cudaStream_t stream) {
     int ctas = 1;  // of a cluster: a power of two that a tile's rows and channels can be shared by
     while (ctas < AT_MAX_CLUSTER && 2 * ctas * tiles <= 2 * sms && 2 * ctas <= (a.K + AT_K - 1) / AT_K) ctas *= 2;
     q.stages = 8;
-    while (q.stages > 2 && adapter_up_smem(q.RP, a.R, q.stages) > 220 * 1024) --q.stages;
+    while (q.stages > 4 && adapter_up_smem(q.RP, a.R, q.stages) > 220 * 1024) --q.stages;
     const size_t down_smem = adapter_down_smem(q.RP), up_smem = adapter_up_smem(q.RP, a.R, q.stages);
     static bool attr_set[64] = {false};
     int dev = 0;
@@ -441,6 +447,7 @@ int adapters_tc(const AdapterParams &a, cudaStream_t stream) {
     cfg.dynamicSmemBytes = down_smem;
     NCKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, adapter_tile_down, map_x, map_down, q));
     cfg.numAttrs = 1;
+    cfg.blockDim = dim3(AT_UP_THREADS);
     cfg.gridDim = dim3((unsigned)(tiles * n_steps < sms ? tiles * n_steps : sms));
     cfg.dynamicSmemBytes = up_smem;
     NCKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, adapter_tile_up, map_t, map_up, map_y, map_out, q));
