@@ -19,7 +19,7 @@ struct AdapterParams {
 };
 
 // The form on the tensor cores: many tokens per request.
-bool adapters_tiled(int T);
+bool adapters_tiled(int B, int T);
 size_t adapters_tc_bytes(int B, int T, int R);
 int adapters_tc(const AdapterParams &p, cudaStream_t stream);
 

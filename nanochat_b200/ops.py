@@ -984,11 +984,12 @@ def _adapters(name, y, x, down, up, slots, scales, out):
     status = workspace(y.device, 1, 1, 1)
     idx = y.device.index
     with _device_guard(idx):
-        # t = down x between the two launches: the call's own (or the graph's that holds it)
+        # t = down x between two launches: the call's own (or the graph's that holds it)
         need = _lib.lib.nckv_adapters_workspace_bytes(B, rows // B, K, N, R, S)
-        scratch = torch.empty(max(need, 1), dtype=torch.uint8, device=y.device)
+        scratch = torch.empty(need, dtype=torch.uint8, device=y.device) if need else None
         _lib.call("nckv_adapters", y.data_ptr(), y_stride, x.data_ptr(), x_stride, down.data_ptr(), up.data_ptr(), slots.data_ptr(),
-                  scales.data_ptr(), (y if out is None else out).data_ptr(), out_stride, B, rows // B, K, N, R, S, scratch.data_ptr(), need,
+                  scales.data_ptr(), (y if out is None else out).data_ptr(), out_stride, B, rows // B, K, N, R, S,
+                  scratch.data_ptr() if need else None, need,
                   status.data_ptr(), torch.cuda.current_stream(idx).cuda_stream)
 
 

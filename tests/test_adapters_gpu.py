@@ -51,6 +51,12 @@ SIZES = [
     (1, 700, 1536, 392, 8, 1),
     (4, 513, 2048, 2048, 32, 3),
     (2, 1100, 200, 4104, 72, 9),
+    # many tokens: tiles of 128
+    (3, 400, 776, 1160, 128, 2),
+    (30, 57, 264, 1032, 24, 4),
+    (9, 129, 8, 8, 8, 3),
+    (5, 256, 6144, 72, 16, 5),
+    (2, 600, 1000, 2056, 48, 1),
 ]
 
 
@@ -69,7 +75,7 @@ def test_matches_definition(B, T, K, N, R, S):
     assert out is args[0] and torch.equal(out, got)
 
 
-@pytest.mark.parametrize("T", [1, 2, 7, 200])
+@pytest.mark.parametrize("T", [1, 2, 7, 200, 260])
 @pytest.mark.parametrize("slots", [[-1] * 5, [2] * 5, [0, -1, 0, 3, -1], [3, 2, 1, 0, 3]])
 def test_who_shares_an_adapter(T, slots):
     from nanochat_b200 import ops
@@ -103,7 +109,7 @@ def test_a_row_does_not_depend_on_its_batch():
     assert torch.equal(got[keep], all_[keep])
 
 
-@pytest.mark.parametrize("T", [1, 150])
+@pytest.mark.parametrize("T", [1, 150, 260])
 def test_column_slices(T):
     from nanochat_b200 import ops
     y, x, down, up, slots, scales = args = make(4, T, 256, 384, 16, 3, seed=4, slots=[0, 2, -1, 1])
@@ -126,7 +132,7 @@ def test_column_slices(T):
 
 def test_a_slot_outside_the_bank():
     from nanochat_b200 import ops
-    for T in (1, 3, 40, 300):
+    for T in (1, 3, 40, 300, 400):
         y, x, down, up, slots, scales = make(3, T, 64, 64, 8, 2, seed=T, slots=[0, 2, 1])
         got = ops.add_adapters(y, x, down, up, slots, scales)
         assert ops.read_status(DEV) == 16
@@ -156,7 +162,7 @@ def test_refusals():
     assert ops.add_adapters(y[:, :0], x[:, :0], down, up, slots, scales).shape == (3, 0, 48)
 
 
-@pytest.mark.parametrize("T", [1, 130])
+@pytest.mark.parametrize("T", [1, 130, 260])
 def test_captured_and_replayed_with_other_slots(T):
     from nanochat_b200 import ops
     first, second = make(4, T, 256, 256, 16, 3, seed=1, slots=[0, 1, 1, -1]), make(4, T, 256, 256, 16, 3, seed=2, slots=[2, -1, 0, 0])
@@ -181,7 +187,7 @@ def test_captured_and_replayed_with_other_slots(T):
 def test_in_two_threads():
     import threading
     from nanochat_b200 import ops
-    args = [make(6, T, 512, 512, 16, 3, seed=T) for T in (1, 90)]
+    args = [make(6, T, 512, 512, 16, 3, seed=T) for T in (1, 200)]
     want = [ops.add_adapters(*a) for a in args]
     torch.cuda.synchronize()
     got = [[], []]
