@@ -8,7 +8,8 @@
 //
 // A tile is CH_M = 128 query rows of one (row, kv head): the G query heads of the group at 128 / G consecutive tokens, row = token * G +
 // head, so keys and values are read once for the whole group.  It walks over its keys in tiles of 64, cut at multiples of 64.  Pages
-// hold a multiple of 48 tokens: a tile is copied in boxes of gcd(64, page) keys, each of which lies in one page.
+// hold a multiple of 48 tokens, so a tile lies in one page or in two, at a multiple of 16: it is copied in one box or two, by maps of boxes of
+// 16, 32, 48 and 64 keys.
 // The pipeline is that of the dense kernel (prefill_attn.cu): two persistent CTAs per SM, a copying thread, a thread that issues S = Q K^T two
 // tiles ahead and O += P V, and one softmax thread per query row that takes its scores out of tensor memory and puts P back over them.
 //
@@ -32,12 +33,17 @@ namespace nckv {
 constexpr int CH_M = 128, CH_N = 64;
 constexpr int CH_STAGES = 2, CH_VSTAGES = 3;  // of K and of V
 constexpr int CH_THREADS = CH_M + 64;         // softmax threads, the issuing warp, the copying warp
-constexpr int CH_Q_BYTES = CH_M * NCKV_D * 2, CH_KV_BYTES = CH_N * NCKV_D * 2;
+constexpr int CH_KV_BYTES = CH_N * NCKV_D * 2;
 constexpr int CH_TMEM_COLS = 256;  // S / P buffers [0, 64), [64, 128); O [128, 256)
 constexpr int CH_PHASES = 4;       // most groups of pairs that are cut one after the other
 constexpr int CH_MIN_TILES = 1;    // shortest stretch of a CTA
+constexpr int CH_ROWS = 8192;      // most rows of a launch: 64 KB of shared memory that the keys come to later
 constexpr int CH_RING = 8;         // pieces of work that the copying thread can be ahead with: it is four at most (five stages, pieces of one tile)
 constexpr long long CH_PART_BYTES = 160LL << 20, CH_PHASE_BYTES = 48LL << 20;
+
+struct ChunkMaps {
+    CUtensorMap q, k[4], v[4];  // k, v: boxes of 16, 32, 48 and 64 keys of 64 channels
+};
 
 struct ChunkPlan {  // a CTA's stretch of a phase: its first key tile (-1: none), how far into which tile of queries that is, and the whole tile's key tiles
     int at, off, count, b, hkv, t0, begin, each;  // the phase begins at `begin` and is cut every `each`
@@ -52,7 +58,7 @@ struct ChunkParams {
     float *part_o;   // (slots, part_rows, 128), not divided by the sum
     int32_t *status;
     int B, T, Hq, Hkv, G, tile_tokens, n_qtiles;
-    int page_tokens, max_pages, n_pages, capacity, box;
+    int page_tokens, max_pages, n_pages, capacity;
     int64_t page_stride, token_stride;
     int window_left;
     int phases, part_rows;        // phases 0: nothing is cut
@@ -236,15 +242,19 @@ __device__ __noinline__ float chunk_not_finite(const ChunkParams &p, const Chunk
     return sum;
 }
 
+__host__ __device__ constexpr uint32_t chunk_q_half(int rows) { return (rows <= 32 ? 32 : rows <= 64 ? 64 : 128) * 128; }
+
 __global__ void __launch_bounds__(CH_THREADS, 2)
-chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
-                  const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ ChunkParams p) {
+chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant__ ChunkParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     if ((smem_u32(smem) & 1023u) != 0) {  // uniform; checked rather than assumed
         if (threadIdx.x == 0) atomicOr(p.status, (int)NCKV_ST_TIMEOUT);
         return;
     }
-    uint8_t *sQ = smem, *sK = sQ + CH_Q_BYTES, *sV = sK + CH_STAGES * CH_KV_BYTES;
+    // Q in one buffer of two halves of 128 rows, or two buffers where a piece has at most 64 or 32 rows (the product reads 128 all the same:
+    // what it finds behind them only reaches rows that nobody looks at)
+    const uint32_t q_bufs = p.part_rows <= CH_M / 2 ? 2 : 1, q_half = chunk_q_half(p.part_rows);
+    uint8_t *sQ = smem, *sK = sQ + 2 * q_bufs * q_half, *sV = sK + CH_STAGES * CH_KV_BYTES;
     // Barriers of key tiles are indexed by the tile's number g in the CTA's stream: stage g % 2 or g % 3, buffer g & 1, and the phase
     // follows from g as well.  (What each of them says: prefill_attn.cu.)
     uint64_t *bars = reinterpret_cast<uint64_t *>(sV + CH_VSTAGES * CH_KV_BYTES);
@@ -255,15 +265,14 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     volatile int *s_poison = reinterpret_cast<volatile int *>(tmem_slot + 2);        // [4]: piece seq (seq & 3) had values that are not finite
     ChunkStretch *s_stretch = reinterpret_cast<ChunkStretch *>(tmem_slot + 6);       // [CH_PHASES]
-    int *s_bound = reinterpret_cast<int *>(s_stretch + CH_PHASES);                   // [CH_PHASES + 1]: key tiles before a phase
     int *s_sum = reinterpret_cast<int *>(ring);                                      // [5][6], before there are pieces
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
-        prefetch_tensormap(&tmap_q);
-        prefetch_tensormap(&tmap_k);
-        prefetch_tensormap(&tmap_v);
+        prefetch_tensormap(&maps.q);
+        prefetch_tensormap(&maps.k[3]);
+        prefetch_tensormap(&maps.v[3]);
         for (int i = 0; i < CH_RING; ++i) mbar_init(&bar_u[i], 1);
         for (int s = 0; s < CH_STAGES; ++s) mbar_init(&bar_k[s], 1);
         for (int s = 0; s < CH_VSTAGES; ++s) mbar_init(&bar_v[s], 1);
@@ -283,30 +292,15 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         tmem_relinquish();
     }
     pdl_wait_prior_grids();  // lengths and tables may come from the grid before
-    // ---- lengths: `width` lanes to a row, a run of rows to each such group of lanes ----------------------
+    // ---- lengths: `width` lanes to a row -----------------------------------------------------------------
+    // s_tiles[b]: key tiles of row b's tiles of queries, per kv head; s_place[b]: key tiles before row b.  They lie where K and V come later.
+    int *s_tiles = reinterpret_cast<int *>(sK), *s_place = s_tiles + CH_ROWS;
     int width = 1;
     while (width < 32 && width < p.n_qtiles) width *= 2;
-    const int member = tid & (width - 1), groups = CH_THREADS / width, group = tid / width;
-    const int run = (p.B + groups - 1) / groups, b_lo = min(group * run, p.B), b_hi = min(b_lo + run, p.B);
-    // key tiles of the row's tiles of queries that this lane counts; per kv head
-    auto my_tiles = [&](const ChunkRow &r, int *longest) {
-        int n = 0;
-        for (int qt = member; qt * p.tile_tokens < r.n; qt += width) {
-            const int c = chunk_span(p, r, qt * p.tile_tokens).count;
-            n += c;
-            if (longest) *longest = max(*longest, c);
-        }
-        return n;
-    };
-    auto row_tiles = [&](const ChunkRow &r) {  // of all the group's lanes
-        int n = my_tiles(r, nullptr);
-        const uint32_t mask = width == 32 ? 0xffffffffu : ((1u << width) - 1) << (lane & ~(width - 1));
-        for (int off = 1; off < width; off <<= 1) n += __shfl_xor_sync(mask, n, off);
-        return n;
-    };
-    int tiles = 0, items = 0, longest = 0, least = 0x7fffffff, most = 0;
+    const int member = tid & (width - 1), groups = CH_THREADS / width;
+    int items = 0, longest = 0, least = 0x7fffffff, most = 0;
     bool idle = false;  // a row has slots without a token, or can't be
-    for (int b = b_lo; b < b_hi; ++b) {
+    for (int b = tid / width; b < p.B; b += groups) {  // (whole groups of lanes)
         const ChunkRow r = chunk_row(p, b);
         idle |= r.n < p.T;
         if (blockIdx.x == 0 && member == 0) {  // lengths out of range: reported once
@@ -314,92 +308,116 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             if (L < 0 || n < 0) atomicOr(p.status, (int)NCKV_ST_BAD_SEQLEN);
             else if (n > p.T || (long long)L + n > p.capacity) atomicOr(p.status, (int)NCKV_ST_OVERFLOW);
         }
-        const int n = my_tiles(r, &longest);
-        tiles += n * p.Hkv;
-        if (member == 0) items += (r.n + p.tile_tokens - 1) / p.tile_tokens * p.Hkv;
-        if (p.n_qtiles > 1) {
-            const long long work = r.n > 0 ? (long long)chunk_span(p, r, (r.n - 1) / p.tile_tokens * p.tile_tokens).count * r.n : 0;
-            const int last = (int)min(work, 0x7fffffffLL);
-            least = min(least, last);
-            most = max(most, last);
+        int n = 0;
+        for (int qt = member; qt * p.tile_tokens < r.n; qt += width) {
+            const int c = chunk_span(p, r, qt * p.tile_tokens).count;
+            n += c;
+            longest = max(longest, c);
+        }
+        const uint32_t mask = width == 32 ? 0xffffffffu : ((1u << width) - 1) << (lane & ~(width - 1));
+        for (int off = 1; off < width; off <<= 1) n += __shfl_xor_sync(mask, n, off);
+        if (member == 0) {
+            s_tiles[b] = n;
+            items += (r.n + p.tile_tokens - 1) / p.tile_tokens * p.Hkv;
+            least = min(least, n);
+            most = max(most, n);
         }
     }
-    int before = tiles;  // inclusive sum over the warp, then over the threads before this one
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, before, off);
-        if (lane >= off) before += v;
-    }
+    __syncwarp();
     items = __reduce_add_sync(0xffffffffu, items);
     longest = __reduce_max_sync(0xffffffffu, longest);
     least = __reduce_min_sync(0xffffffffu, least);
     most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 31) {
-        s_sum[warp] = before;
-        s_sum[6 + warp] = items;
-        s_sum[12 + warp] = longest;
-        s_sum[18 + warp] = least;
-        s_sum[24 + warp] = most;
+    if (lane == 0) {
+        s_sum[warp] = items;
+        s_sum[6 + warp] = longest;
+        s_sum[12 + warp] = least;
+        s_sum[18 + warp] = most;
     }
     tc_fence_before();
     const bool any_idle = __syncthreads_or(idle);
     tc_fence_after();
-    int all = 0;
-    before -= tiles;
     items = 0;
     for (int w = 0; w < CH_THREADS / 32; ++w) {
-        if (w < warp) before += s_sum[w];
-        all += s_sum[w];
-        items += s_sum[6 + w];
-        longest = max(longest, s_sum[12 + w]);
-        least = min(least, s_sum[18 + w]);
-        most = max(most, s_sum[24 + w]);
+        items += s_sum[w];
+        longest = max(longest, s_sum[6 + w]);
+        least = min(least, s_sum[12 + w]);
+        most = max(most, s_sum[18 + w]);
     }
-    before = __shfl_sync(0xffffffffu, before, lane & ~(width - 1));  // of the group's first lane: tiles before its rows
+    int all = 0;  // key tiles before a chunk of rows, then of all
+    for (int b0 = 0; b0 < p.B; b0 += CH_THREADS) {
+        const int mine = b0 + tid < p.B ? s_tiles[b0 + tid] * p.Hkv : 0;
+        int before = mine;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, before, off);
+            if (lane >= off) before += v;
+        }
+        if (b0) __syncthreads();  // the sums of the chunk before have been read
+        if (lane == 31) s_sum[24 + warp] = before;
+        __syncthreads();
+        before += all - mine;
+        for (int w = 0; w < CH_THREADS / 32; ++w) {
+            if (w < warp) before += s_sum[24 + w];
+            all += s_sum[24 + w];
+        }
+        if (b0 + tid < p.B) s_place[b0 + tid] = before;
+    }
     const bool dealt = chunk_dealt(p, least, most, all, items, longest, (int)gridDim.x);
     if (tid < p.phases) p.plan[tid * gridDim.x + blockIdx.x].at = -1;
-    if (!dealt) {
-        // where the phases begin
-        if (tid == 0) s_bound[p.phases] = all;
-        for (int b = b_lo, base = before; b < b_hi; ++b) {
-            const ChunkRow r = chunk_row(p, b);
-            const int n = row_tiles(r);
-            for (int f = 0; f < p.phases; ++f) {
-                const int pair = f * p.phase_pairs - b * p.Hkv;
-                if (member == 0 && pair >= 0 && pair < p.Hkv) s_bound[f] = base + pair * n;
+    __syncthreads();
+    // A warp to a phase: its stretch of this CTA.
+    if (!dealt && warp < p.phases) {
+        auto place = [&](int pair) {  // key tiles before a (row, kv head)
+            const int b = pair / p.Hkv;
+            return b < p.B ? s_place[b] + (pair - b * p.Hkv) * s_tiles[b] : all;
+        };
+        const int lo = place(warp * p.phase_pairs), hi = place(min((warp + 1) * p.phase_pairs, p.B * p.Hkv));
+        const int each = max((hi - lo + (int)gridDim.x - 1) / (int)gridDim.x, CH_MIN_TILES);
+        const int from = (int)min(lo + (long long)each * blockIdx.x, (long long)hi);
+        if (from < hi) {
+            int row = -1;
+            for (int b0 = 0; row < 0; b0 += 32) {  // the row that holds key tile `from`
+                const int b = b0 + lane;
+                const unsigned votes = __ballot_sync(0xffffffffu, b < p.B && s_place[b] <= from && from < s_place[b] + s_tiles[b] * p.Hkv);
+                if (votes) row = b0 + __ffs(votes) - 1;
             }
-            base += n * p.Hkv;
-        }
-        __syncthreads();
-        for (int f = 0; f < p.phases; ++f) {
-            const int lo = s_bound[f], hi = s_bound[f + 1];
-            const int each = p.phases == 1 && gridDim.x == 1 ? max(hi - lo, 1) : max((hi - lo + (int)gridDim.x - 1) / (int)gridDim.x, CH_MIN_TILES);
-            const int from = (int)min(lo + (long long)each * blockIdx.x, (long long)hi);
-            if (from >= hi) continue;
-            for (int b = b_lo, base = before; b < b_hi && base <= from; ++b) {
-                const ChunkRow r = chunk_row(p, b);
-                const int n = row_tiles(r), rel = from - base;
-                base += n * p.Hkv;
-                if (from >= base || member) continue;
-                ChunkStretch st;
-                st.at = from;
-                st.end = min(from + each, hi);
-                st.b = b;
-                st.hkv = rel / n;
-                st.off = rel - st.hkv * n;
-                st.qt = 0;
-                int count;
-                for (;; ++st.qt) {
-                    count = chunk_span(p, r, st.qt * p.tile_tokens).count;
-                    if (st.off < count) break;
-                    st.off -= count;
+            const ChunkRow r = chunk_row(p, row);
+            ChunkStretch st;
+            st.at = from;
+            st.end = min(from + each, hi);
+            st.b = row;
+            const int rel = from - s_place[row];
+            st.hkv = rel / s_tiles[row];
+            int off = rel - st.hkv * s_tiles[row], count = 0;
+            for (int qt0 = 0;; qt0 += 32) {  // and the tile of queries
+                count = chunk_span(p, r, (qt0 + lane) * p.tile_tokens).count;
+                int upto = count;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, upto, d);
+                    if (lane >= d) upto += v;
                 }
-                s_stretch[f] = st;
-                if (p.phases) p.plan[f * gridDim.x + blockIdx.x] = ChunkPlan{st.at, st.off, count, b, st.hkv, st.qt * p.tile_tokens, lo, each};
+                const unsigned votes = __ballot_sync(0xffffffffu, off < upto);
+                if (votes) {
+                    const int l = __ffs(votes) - 1;
+                    off -= __shfl_sync(0xffffffffu, upto - count, l);
+                    count = __shfl_sync(0xffffffffu, count, l);
+                    st.qt = qt0 + l;
+                    break;
+                }
+                off -= __shfl_sync(0xffffffffu, upto, 31);
+            }
+            st.off = off;
+            if (lane == 0) {
+                s_stretch[warp] = st;
+                p.plan[warp * gridDim.x + blockIdx.x] = ChunkPlan{st.at, off, count, row, st.hkv, st.qt * p.tile_tokens, lo, each};
             }
         }
     }
+    fence_proxy_async_smem();  // the sums' place is K's from here on
     __syncthreads();
+    pdl_launch_dependents();  // the sums of parts: their CTAs wait where there is room for them
     const uint32_t tmem_base = *tmem_slot;
     const uint32_t tmem_s = tmem_base, tmem_o = tmem_base + 128;
     const uint32_t lane_sel = (uint32_t)((warp & 3) * 32) << 16;  // a warp reaches TMEM lanes 32*(warp % 4) ..
@@ -411,9 +429,6 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         atomicOr(p.status, (int)NCKV_ST_TIMEOUT);
     };
     auto par2 = [](uint32_t g) -> uint32_t { return (g >> 1) & 1u; };
-    // Q in one buffer of two halves of 128 rows, or two buffers where a piece has at most 64 rows (the product reads 128 all the same:
-    // what it finds behind them only reaches rows that nobody looks at)
-    const uint32_t q_bufs = p.part_rows <= CH_M / 2 ? 2 : 1, q_half = CH_Q_BYTES / 2 / q_bufs;
 
     if (warp == CH_M / 32 + 1) {
         // =============== one lane moves the tiles ===================================================
@@ -428,50 +443,58 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
                 mbar_arrive(&bar_u[nu % CH_RING]);
                 ++nu;
             };
-            // The places of a tile's boxes, looked up a tile ahead of its copies.  Boxes outside [kv_lo, kv_hi) need no page: they read as
-            // zeros, as pages outside the pool do.
+            // Where a tile lies, looked up a tile ahead of its copies: `keys` of it in one page, the rest at the next one's front.  Parts outside
+            // [kv_lo, kv_hi) need no page: they read as zeros, as pages outside the pool do.
             struct Places {
-                int idx, tok;  // page of the row and token in it at which the next tile begins
-                int page[4], at[4], need;
+                int idx, tok;  // page of the row, and token in it at which the tile begins
+                int page[2], need, keys;
             };
             auto look_up = [&](Places &pl, const ChunkUnit &u, int t) {
                 const int key0 = (u.tile0 + t) * CH_N;
                 if (t == 0) {
                     pl.idx = key0 / p.page_tokens;
                     pl.tok = key0 - pl.idx * p.page_tokens;
-                }
-                pl.need = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = key0 + i * p.box;
-                    if (i * p.box >= CH_N) break;
-                    pl.at[i] = pl.tok;
-                    if (key < u.kv_hi && key + p.box > u.kv_lo) {
-                        pl.page[i] = __ldg(p.table + (long long)u.b * p.max_pages + pl.idx);
-                        pl.need |= 1 << i;
-                    }
-                    pl.tok += p.box;
+                } else {
+                    pl.tok += CH_N;
                     if (pl.tok >= p.page_tokens) {
                         pl.tok -= p.page_tokens;
                         ++pl.idx;
                     }
+                    if (pl.tok >= p.page_tokens) {  // pages of 48
+                        pl.tok -= p.page_tokens;
+                        ++pl.idx;
+                    }
+                }
+                pl.keys = min(CH_N, p.page_tokens - pl.tok);
+                const int32_t *row = p.table + (long long)u.b * p.max_pages + pl.idx;
+                pl.need = 0;
+                if (key0 + pl.keys > u.kv_lo) {  // key0 < kv_hi for every tile
+                    pl.page[0] = __ldg(row);
+                    pl.need = 1;
+                }
+                if (pl.keys < CH_N && key0 + pl.keys < u.kv_hi) {  // and its last key is one of the piece's or behind them
+                    pl.page[1] = __ldg(row + 1);
+                    pl.need |= 2;
                 }
             };
             auto load_tile = [&](uint8_t *dst, const CUtensorMap *map, uint64_t *bar, const Places &pl, int hkv) {
                 mbar_arrive_expect_tx(bar, CH_KV_BYTES);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (i * p.box >= CH_N) break;
-                    int page = p.n_pages;
-                    if (pl.need >> i & 1) {
-                        page = pl.page[i];
-                        if (page < 0 || page >= p.n_pages) {
-                            atomicOr(p.status, (int)NCKV_ST_BAD_PAGE);
-                            page = p.n_pages;
-                        }
-                    }
-                    tma_load_4d(dst + i * p.box * 128, map, bar, 0, hkv, pl.at[i], page);
-                    tma_load_4d(dst + CH_KV_BYTES / 2 + i * p.box * 128, map, bar, 64, hkv, pl.at[i], page);
+                int page0 = p.n_pages, page1 = p.n_pages;
+                if (pl.need & 1) page0 = pl.page[0];
+                if (pl.need & 2) page1 = pl.page[1];
+                if (((pl.need & 1) && (unsigned)page0 >= (unsigned)p.n_pages) || ((pl.need & 2) && (unsigned)page1 >= (unsigned)p.n_pages)) {
+                    atomicOr(p.status, (int)NCKV_ST_BAD_PAGE);
+                    page0 = min((unsigned)page0, (unsigned)p.n_pages);
+                    page1 = min((unsigned)page1, (unsigned)p.n_pages);
+                }
+                const CUtensorMap *m = map + (pl.keys / 16 - 1);
+                tma_load_4d(dst, m, bar, 0, hkv, pl.tok, page0);
+                tma_load_4d(dst + CH_KV_BYTES / 2, m, bar, 64, hkv, pl.tok, page0);
+                if (pl.keys < CH_N) {
+                    m = map + (CH_N - pl.keys) / 16 - 1;
+                    dst += pl.keys * 128;
+                    tma_load_4d(dst, m, bar, 0, hkv, 0, page1);
+                    tma_load_4d(dst + CH_KV_BYTES / 2, m, bar, 64, hkv, 0, page1);
                 }
             };
             Places kp, vp;
@@ -480,7 +503,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             bool v_known = true;  // its places
             auto load_k = [&]() {
                 const int stage = (int)(gk % CH_STAGES);
-                load_tile(sK + stage * CH_KV_BYTES, &tmap_k, &bar_k[stage], kp, kc.u.hkv);
+                load_tile(sK + stage * CH_KV_BYTES, maps.k, &bar_k[stage], kp, kc.u.hkv);
                 const bool ends = kc.last_of_unit();
                 kc.advance(p, s_stretch);
                 ++gk;
@@ -491,7 +514,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
                 const int stage = (int)(gv % CH_VSTAGES);
                 const ChunkUnit &u = ring[vu % CH_RING];
                 if (!v_known) look_up(vp, u, vt);
-                load_tile(sV + stage * CH_KV_BYTES, &tmap_v, &bar_v[stage], vp, u.hkv);
+                load_tile(sV + stage * CH_KV_BYTES, maps.v, &bar_v[stage], vp, u.hkv);
                 ++gv;
                 if (++vt == u.n_tiles) {
                     vt = 0;
@@ -503,10 +526,10 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             auto load_q = [&]() {
                 const ChunkUnit &u = ring[nq % CH_RING];
                 const uint32_t buf = nq % q_bufs;
-                uint8_t *dst = sQ + buf * (CH_Q_BYTES / 2);
+                uint8_t *dst = sQ + 2 * buf * q_half;
                 mbar_arrive_expect_tx(&bar_q[buf], (uint32_t)(p.tile_tokens * p.G * NCKV_D * 2));
-                tma_load_4d(dst, &tmap_q, &bar_q[buf], 0, u.hkv * p.G, u.t0, u.b);
-                tma_load_4d(dst + q_half, &tmap_q, &bar_q[buf], 64, u.hkv * p.G, u.t0, u.b);
+                tma_load_4d(dst, &maps.q, &bar_q[buf], 0, u.hkv * p.G, u.t0, u.b);
+                tma_load_4d(dst + q_half, &maps.q, &bar_q[buf], 64, u.hkv * p.G, u.t0, u.b);
                 ++nq;
             };
             bool ok = true;
@@ -567,7 +590,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 #pragma unroll
                 for (int kk = 0; kk < NCKV_D / 16; ++kk) {
                     const uint32_t off = (uint32_t)(kk & 3) * 32;
-                    const uint64_t da = desc_q + (uint64_t)((buf * (CH_Q_BYTES / 2) + (kk >> 2) * q_half + off) >> 4);
+                    const uint64_t da = desc_q + (uint64_t)(((2 * buf + (kk >> 2)) * q_half + off) >> 4);
                     const uint64_t db = dk + (uint64_t)(((kk >> 2) * (CH_KV_BYTES / 2) + off) >> 4);
                     umma_bf16(ds, da, db, IDESC_S, kk > 0 ? 1u : 0u);
                 }
@@ -810,9 +833,9 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 }
 
 // Adds up the parts of a tile of queries whose keys were cut: O = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s.  Block (CTA, rows, phase) looks at
-// the cut where that CTA's stretch begins and takes the tile's rows if it is the tile's first cut; WARPS warps to a row.
-constexpr int CH_FINISH_ROWS = 4;  // of a warp
-template <int WARPS>
+// the cut where that CTA's stretch begins and takes the tile's rows if it is the tile's first cut; WARPS warps to a row, EACH rows
+// one after the other.
+template <int WARPS, int EACH>
 __global__ void __launch_bounds__(256) chunk_finish_kernel(const __grid_constant__ ChunkParams p) {
     pdl_wait_prior_grids();
     __shared__ float4 s_o[WARPS > 1 ? 8 : 1][32];
@@ -828,9 +851,9 @@ __global__ void __launch_bounds__(256) chunk_finish_kernel(const __grid_constant
     const bool second = first * cut.each < from;  // the first part is not the first piece of its stretch
     auto part_of = [&](int i, int row) -> long long { return (slot0 + 2 * i + (i == 0 && second)) * p.part_rows + row; };
     constexpr int STEP = 8 / WARPS;
-    const int row0 = (int)blockIdx.y * STEP * (WARPS > 1 ? 1 : CH_FINISH_ROWS) + warp / WARPS;
+    const int row0 = (int)blockIdx.y * STEP * EACH + warp / WARPS;
 #pragma unroll 1
-    for (int k = 0; k < (WARPS > 1 ? 1 : CH_FINISH_ROWS); ++k) {
+    for (int k = 0; k < EACH; ++k) {
         const int row = row0 + k * STEP;
         if (row >= rows) return;  // uniform over the warps of a row
         float m = -INFINITY, l = 0.f;
@@ -873,9 +896,9 @@ __global__ void __launch_bounds__(256) chunk_finish_kernel(const __grid_constant
     }
 }
 
-static size_t chunk_smem_bytes() {
-    return CH_Q_BYTES + (CH_STAGES + CH_VSTAGES) * CH_KV_BYTES + (13 + CH_RING) * sizeof(uint64_t) + CH_RING * sizeof(ChunkUnit) + 6 * 4 +
-           CH_PHASES * sizeof(ChunkStretch) + (CH_PHASES + 1) * 4;
+static size_t chunk_smem_bytes(int part_rows) {
+    return 2 * (part_rows <= CH_M / 2 ? 2 : 1) * chunk_q_half(part_rows) + (CH_STAGES + CH_VSTAGES) * CH_KV_BYTES + (13 + CH_RING) * sizeof(uint64_t) + CH_RING * sizeof(ChunkUnit) + 6 * 4 +
+           CH_PHASES * sizeof(ChunkStretch);
 }
 static_assert(CH_RING * sizeof(ChunkUnit) >= 30 * 4, "the sums over the rows lie where the pieces come later");
 
@@ -917,6 +940,10 @@ static int chunk_check_sizes(const char *name, int B, int T, int Hq, int Hkv, in
     if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || page_tokens <= 0 || max_pages <= 0) {
         set_error("%s: non-positive size (B=%d T=%d Hq=%d Hkv=%d page_tokens=%d max_pages=%d)", name, B, T, Hq, Hkv, page_tokens, max_pages);
         return NCKV_E_ARG;
+    }
+    if (B > CH_ROWS) {
+        set_error("%s: B=%d rows, at most %d", name, B, CH_ROWS);
+        return NCKV_E_UNSUPPORTED;
     }
     if (Hq % Hkv != 0 || Hq / Hkv > CH_M) {
         set_error("%s: Hq=%d must be a multiple of Hkv=%d, at most %d times it", name, Hq, Hkv, CH_M);
@@ -974,16 +1001,15 @@ extern "C" int nckv_prefill_attn_paged(const void *q, const void *k_pool, const 
         set_error("%s: needs %zu bytes of workspace, 256-byte aligned", name, need);
         return workspace && workspace_bytes < need ? NCKV_E_CAPACITY : NCKV_E_ARG;
     }
-    int box = CH_N;
-    while (page_tokens % box) box /= 2;  // 16 at least: pages are multiples of 48
-    CUtensorMap mq, mk, mv;
+    ChunkMaps maps;
     const int64_t dims[4] = {D, Hq, T, B}, strides[3] = {D, (int64_t)Hq * D, (int64_t)T * Hq * D};
     const int q_box[4] = {64, s.G, s.tile_tokens, 1};
-    rc = make_tensor_map(&mq, q, 4, dims, strides, q_box);
-    if (rc != NCKV_OK) return rc;
-    rc = make_kv_tensor_map(&mk, k_pool, n_pages, page_tokens, Hkv, page_stride, token_stride, box);
-    if (rc != NCKV_OK) return rc;
-    rc = make_kv_tensor_map(&mv, v_pool, n_pages, page_tokens, Hkv, page_stride, token_stride, box);
+    rc = make_tensor_map(&maps.q, q, 4, dims, strides, q_box);
+    for (int i = 0; i < 4 && rc == NCKV_OK; ++i) {
+        if (i < 3 && page_tokens % CH_N == 0) continue;  // tiles lie in one page
+        rc = make_kv_tensor_map(&maps.k[i], k_pool, n_pages, page_tokens, Hkv, page_stride, token_stride, 16 * (i + 1));
+        if (rc == NCKV_OK) rc = make_kv_tensor_map(&maps.v[i], v_pool, n_pages, page_tokens, Hkv, page_stride, token_stride, 16 * (i + 1));
+    }
     if (rc != NCKV_OK) return rc;
 
     ChunkParams p;
@@ -1000,7 +1026,7 @@ extern "C" int nckv_prefill_attn_paged(const void *q, const void *k_pool, const 
     }
     p.status = status;
     p.B = B; p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.G = s.G; p.tile_tokens = s.tile_tokens; p.n_qtiles = s.n_qtiles;
-    p.page_tokens = page_tokens; p.max_pages = max_pages; p.n_pages = n_pages; p.capacity = page_tokens * max_pages; p.box = box;
+    p.page_tokens = page_tokens; p.max_pages = max_pages; p.n_pages = n_pages; p.capacity = page_tokens * max_pages;
     p.page_stride = page_stride; p.token_stride = token_stride;
     p.window_left = window_left;
     p.phases = s.phases; p.phase_pairs = s.phase_pairs; p.part_rows = s.part_rows;
@@ -1023,12 +1049,12 @@ extern "C" int nckv_prefill_attn_paged(const void *q, const void *k_pool, const 
         p.n_groups = (int)(pairs / g);  // the last group also takes the remainder
         p.group_pairs = (int)g;
     }
-    const size_t smem = chunk_smem_bytes();
+    const size_t smem = chunk_smem_bytes(s.part_rows);
     static bool attr_set[64] = {false};
     int dev = 0;
     NCKV_CUDA_CHECK(cudaGetDevice(&dev));
     if (dev >= 64 || !attr_set[dev]) {
-        NCKV_CUDA_CHECK(cudaFuncSetAttribute(chunk_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        NCKV_CUDA_CHECK(cudaFuncSetAttribute(chunk_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)chunk_smem_bytes(CH_M)));
         if (dev < 64) attr_set[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
@@ -1041,15 +1067,15 @@ extern "C" int nckv_prefill_attn_paged(const void *q, const void *k_pool, const 
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    NCKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, chunk_attn_kernel, mq, mk, mv, p));
+    NCKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, chunk_attn_kernel, maps, p));
     if (s.phases) {
         // few rows: all of a block's warps to one, over the parts
         const bool wide = s.part_rows <= 16;
-        const int step = wide ? 1 : 8 * CH_FINISH_ROWS;
+        const int step = wide ? 1 : s.part_rows <= 64 ? 8 : 16;
         cfg.gridDim = dim3((unsigned)s.grid, (unsigned)((s.part_rows + step - 1) / step), (unsigned)s.phases);
         cfg.blockDim = dim3(256);
         cfg.dynamicSmemBytes = 0;
-        NCKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, wide ? chunk_finish_kernel<8> : chunk_finish_kernel<1>, p));
+        NCKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, wide ? chunk_finish_kernel<8, 1> : step == 8 ? chunk_finish_kernel<1, 1> : chunk_finish_kernel<1, 2>, p));
     }
     return NCKV_OK;
 }
