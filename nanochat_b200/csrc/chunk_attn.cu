@@ -17,8 +17,8 @@
 //   stretches: the sequence of all key tiles of all tiles of queries, (row, kv head) by (row, kv head), is cut into equal stretches, one per
 //     CTA; tiles of queries that lie in several leave partial sums.  Balanced to a key tile whatever the lengths.  Where tiles of queries share
 //     keys (more than one per row) and the keys are more than L2 holds, up to CH_PHASES groups of pairs are cut one after the other.
-//   a deal: tiles of queries of rows of like lengths, enough of them to fill the CTAs' rounds, go to the CTAs uncut, longest first, back and
-//     forth, as in the dense kernel.
+//   a deal: where tiles of queries are many or alike enough to fill the CTAs' rounds they go to the CTAs uncut, back and forth: of rows of like
+//     lengths longest first as in the dense kernel, of others row by row, empty ones left out.
 // chunk_finish_kernel adds up partial sums in the order of the keys: results don't depend on timing.
 //
 // Every barrier wait is bounded; one that runs out sets NCKV_ST_TIMEOUT, the CTA stops issuing work, waits for its copies, frees its
@@ -110,9 +110,9 @@ struct ChunkCursor {
     int t;    // key tile inside the piece
     int seq;  // number of the piece among the CTA's
     bool valid;
-    int phase;  // -1: dealt
+    int phase;  // -1: dealt, -2: dealt row by row
     int at;     // next key tile of the stretch, or next round of the deal
-    int begin, end, qt, off;
+    int begin, end, qt, off;  // (dealt row by row: row `end`, and the tiles of queries before it)
     ChunkSpan span;
 
     __device__ __forceinline__ void item(const ChunkParams &p) {
@@ -140,12 +140,13 @@ struct ChunkCursor {
         }
         return false;
     }
-    __device__ __forceinline__ void start(const ChunkParams &p, const ChunkStretch *stretches, bool dealt) {
+    __device__ __forceinline__ void start(const ChunkParams &p, const ChunkStretch *stretches, int dealt) {
         seq = -1;
         valid = true;
         at = end = begin = 0;
-        phase = dealt ? -1 : 0;
+        phase = -dealt;
         if (!dealt) valid = enter(p, stretches);
+        if (dealt == 2) row(p, 0);
         if (valid) load(p, stretches);
     }
     __device__ __forceinline__ void load(const ChunkParams &p, const ChunkStretch *stretches) {
@@ -187,13 +188,28 @@ struct ChunkCursor {
                 valid = false;
                 return;
             }
-            const int grp = min((int)idx / per_group, p.n_groups - 1), in_grp = (int)idx - grp * per_group;
-            const int grp_pairs = grp == p.n_groups - 1 ? pairs - grp * p.group_pairs : p.group_pairs;
-            const int pair = grp * p.group_pairs + in_grp % grp_pairs;
-            qt = p.n_qtiles - 1 - in_grp / grp_pairs;  // all pairs' longest tiles first
-            row(p, pair / p.Hkv);
-            if (qt * p.tile_tokens >= u.n) continue;
-            u.hkv = pair - u.b * p.Hkv;
+            if (phase == -2) {
+                int tiles;  // of queries, of one kv head of the row
+                while (tiles = (u.n + p.tile_tokens - 1) / p.tile_tokens, idx >= begin + tiles * p.Hkv) {
+                    begin += tiles * p.Hkv;
+                    if (++end == p.B) {
+                        valid = false;
+                        return;
+                    }
+                    row(p, end);
+                }
+                const int local = (int)idx - begin;
+                qt = tiles - 1 - local / p.Hkv;
+                u.hkv = local % p.Hkv;
+            } else {
+                const int grp = min((int)idx / per_group, p.n_groups - 1), in_grp = (int)idx - grp * per_group;
+                const int grp_pairs = grp == p.n_groups - 1 ? pairs - grp * p.group_pairs : p.group_pairs;
+                const int pair = grp * p.group_pairs + in_grp % grp_pairs;
+                qt = p.n_qtiles - 1 - in_grp / grp_pairs;  // all pairs' longest tiles first
+                row(p, pair / p.Hkv);
+                if (qt * p.tile_tokens >= u.n) continue;
+                u.hkv = pair - u.b * p.Hkv;
+            }
             item(p);
             u.kv_lo = span.kv_lo;
             u.kv_hi = span.kv_hi;
@@ -210,15 +226,21 @@ struct ChunkCursor {
     __device__ __forceinline__ bool last_of_unit() const { return t == u.n_tiles - 1; }
 };
 
-// Whether uncut tiles dealt to the CTAs take less than stretches: rows' key tiles per kv head between `least` and `most`, `items` tiles of
-// queries of `tiles` key tiles altogether.  A partial sum of 128 rows (64 KB written and read) costs some 3 tiles, a piece 2.
-__device__ __forceinline__ bool chunk_dealt(const ChunkParams &p, int least, int most, long long tiles, int items, int longest, int grid) {
-    if (p.phases == 0) return true;
-    if (p.n_qtiles == 1 || items < grid || most - least > most / 8) return false;
+// Whether uncut tiles dealt to the CTAs take less than stretches (0): 1 in the order of like rows, 2 row by row.  Rows' key tiles per kv head lie
+// between `least` and `most`; `items` tiles of queries have `tiles` key tiles altogether.  A piece costs some 2 tiles, a phase of stretches
+// CH_CUT for the partial sums that it leaves (twice 64 KB per CTA, written and read) and the launch that adds them up.  us as stretches / like
+// rows / row by row, window -1: 8 x 2048 tokens, 12 + 12 heads, no context 215 / 126 / 170; 2 x 1722, 10 + 1 heads 52 / 37 / 40; 8 x 862, 10 + 1, contexts of
+// 0 to 114 67 / 38 / 47; 2011 behind 60000, 16 + 4 1088 / 1139 / 1147; up to 1931 new tokens in 5 rows, 6 + 6 50 / 45 / 39; 24 x up to 384, 16 + 4, window 1024
+// 113 / 103 / 85; 21 x up to 220 behind up to 3019, 12 + 12 91 / 100 / 99.
+constexpr float CH_CUT = 25.f;
+__device__ __forceinline__ int chunk_dealt(const ChunkParams &p, int least, int most, long long tiles, int items, int longest, int grid) {
+    if (p.phases == 0) return 1;
+    if (p.n_qtiles == 1 || items == 0) return 0;
     const float each = (float)tiles / items, per_cta = (float)tiles / grid, rounds = (float)items / grid;
-    const bool alike = longest < 1.5f * each;  // then rounds are whole, else the short tiles fill them up
-    const float deal = alike ? ceilf(rounds) * (each + 2.f) : fmaxf(per_cta * 1.05f, (float)longest) + 2.f * rounds;
-    return deal <= per_cta + 2.f * rounds + 7.f * p.phases;
+    const bool like_rows = !p.new_tokens && most - least <= most / 3;
+    const bool alike = longest < 1.5f * each;  // then rounds are whole, else the short tiles fill them up, longest first or not
+    const float deal = alike ? ceilf(rounds) * (each + 2.f) : like_rows ? fmaxf(per_cta * 1.05f, (float)longest) + 2.f * rounds : per_cta + longest + 2.f * rounds;
+    return deal <= per_cta + 2.f * rounds + CH_CUT * p.phases ? 2 - like_rows : 0;
 }
 
 __device__ __forceinline__ bool not_finite2(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
@@ -363,7 +385,7 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
         }
         if (b0 + tid < p.B) s_place[b0 + tid] = before;
     }
-    const bool dealt = chunk_dealt(p, least, most, all, items, longest, (int)gridDim.x);
+    const int dealt = chunk_dealt(p, least, most, all, items, longest, (int)gridDim.x);
     if (tid < p.phases) p.plan[tid * gridDim.x + blockIdx.x].at = -1;
     __syncthreads();
     // A warp to a phase: its stretch of this CTA.
@@ -689,10 +711,12 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
                     tmem_ld64(tmem_s_it + lane_sel, s_val);
                     if (edge) {
                         // this row sees columns [c_lo, c_hi) of the tile
-                        const int c_hi = min(pos, it.kv_hi - 1) - key0 + 1;
-                        const int c_lo = p.window_left >= 0 ? pos - p.window_left - key0 : 0;
+                            const int c_hi = min(max(min(pos, it.kv_hi - 1) - key0 + 1, 0), CH_N);
+                            const int c_lo = p.window_left >= 0 ? min(max(pos - p.window_left - key0, 0), CH_N) : 0;
+                            const unsigned long long seen = (c_hi == CH_N ? ~0ull : (1ull << c_hi) - 1) & (c_lo == CH_N ? 0ull : ~0ull << c_lo);
+                            const uint32_t seen0 = (uint32_t)seen, seen1 = (uint32_t)(seen >> 32);
 #pragma unroll
-                        for (int c = 0; c < CH_N; ++c) s_val[c] = (c >= c_lo && c < c_hi) ? s_val[c] : -INFINITY;
+                            for (int c = 0; c < CH_N; ++c) s_val[c] = ((c < 32 ? seen0 : seen1) >> (c & 31) & 1u) ? s_val[c] : -INFINITY;
                     }
                     float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
