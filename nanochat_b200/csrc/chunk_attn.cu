@@ -19,6 +19,8 @@
 //     keys (more than one per row) and the keys are more than L2 holds, up to CH_PHASES groups of pairs are cut one after the other.
 //   a deal: where tiles of queries are many or alike enough to fill the CTAs' rounds they go to the CTAs uncut, back and forth: of rows of like
 //     lengths longest first as in the dense kernel, of others row by row, empty ones left out.
+//   clusters: few pairs of short rows, one tile of queries each, are bound by launches and round trips.  A cluster takes a pair, each CTA a part of its
+//     keys, and the parts meet in shared memory: no sums over the rows ahead of the work, no launch behind it.
 // chunk_finish_kernel adds up partial sums in the order of the keys: results don't depend on timing.
 //
 // Every barrier wait is bounded; one that runs out sets NCKV_ST_TIMEOUT, the CTA stops issuing work, waits for its copies, frees its
@@ -39,6 +41,7 @@ constexpr int CH_PHASES = 4;       // most groups of pairs that are cut one afte
 constexpr int CH_MIN_TILES = 1;    // shortest stretch of a CTA
 constexpr int CH_ROWS = 8192;      // most rows of a launch: 64 KB of shared memory that the keys come to later
 constexpr int CH_RING = 8;         // pieces of work that the copying thread can be ahead with: it is four at most (five stages, pieces of one tile)
+constexpr int CH_PITCH = NCKV_D + 4;  // floats of a row where a cluster's parts meet
 constexpr long long CH_PART_BYTES = 160LL << 20, CH_PHASE_BYTES = 48LL << 20;
 
 struct ChunkMaps {
@@ -266,6 +269,7 @@ __device__ __noinline__ float chunk_not_finite(const ChunkParams &p, const Chunk
 
 __host__ __device__ constexpr uint32_t chunk_q_half(int rows) { return (rows <= 32 ? 32 : rows <= 64 ? 64 : 128) * 128; }
 
+template <bool CLUSTER>
 __global__ void __launch_bounds__(CH_THREADS, 2)
 chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant__ ChunkParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -314,6 +318,40 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
         tmem_relinquish();
     }
     pdl_wait_prior_grids();  // lengths and tables may come from the grid before
+    int dealt = 0;
+    bool any_idle = false;
+    [[maybe_unused]] ChunkUnit mine;
+    // where a cluster's parts meet: where K and V have been
+    [[maybe_unused]] float *s_part = reinterpret_cast<float *>(sK);
+    [[maybe_unused]] float2 *s_part_ml = reinterpret_cast<float2 *>(s_part + CH_M * CH_PITCH);
+    if constexpr (CLUSTER) {
+    const int ctas = (int)cluster_ctas(), rank = (int)cluster_rank(), pair = (int)blockIdx.x / ctas;
+    mine.b = pair / p.Hkv;
+    mine.hkv = pair - mine.b * p.Hkv;
+    mine.t0 = 0;
+    const ChunkRow r = chunk_row(p, mine.b);
+    const ChunkSpan sp = chunk_span(p, r, 0);
+    const int lo = sp.count * rank / ctas;
+    mine.L = r.L;
+    mine.n = r.n;
+    mine.kv_lo = sp.kv_lo;
+    mine.kv_hi = sp.kv_hi;
+    mine.tile0 = sp.first + lo;
+    mine.n_tiles = sp.count * (rank + 1) / ctas - lo;
+    mine.slot = 0;
+    if (tid == 0 && rank == 0 && mine.hkv == 0) {  // lengths out of range: reported once
+        const int L = p.seqlens[mine.b], n = p.new_tokens ? p.new_tokens[mine.b] : p.T;
+        if (L < 0 || n < 0) atomicOr(p.status, (int)NCKV_ST_BAD_SEQLEN);
+        else if (n > p.T || (long long)L + n > p.capacity) atomicOr(p.status, (int)NCKV_ST_OVERFLOW);
+    }
+    for (int t = r.n + rank; t < p.T; t += ctas)  // slots without a token
+        for (int i = tid; i < p.G * 16; i += CH_THREADS)
+            reinterpret_cast<uint4 *>(p.out + (((long long)mine.b * p.T + t) * p.Hq + mine.hkv * p.G) * NCKV_D)[i] = make_uint4(0, 0, 0, 0);
+    if (mine.n_tiles == 0 && tid < CH_M) s_part_ml[tid] = make_float2(-INFINITY, 0.f);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    } else {
     // ---- lengths: `width` lanes to a row -----------------------------------------------------------------
     // s_tiles[b]: key tiles of row b's tiles of queries, per kv head; s_place[b]: key tiles before row b.  They lie where K and V come later.
     int *s_tiles = reinterpret_cast<int *>(sK), *s_place = s_tiles + CH_ROWS;
@@ -357,7 +395,7 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
         s_sum[18 + warp] = most;
     }
     tc_fence_before();
-    const bool any_idle = __syncthreads_or(idle);
+    any_idle = __syncthreads_or(idle);
     tc_fence_after();
     items = 0;
     for (int w = 0; w < CH_THREADS / 32; ++w) {
@@ -385,7 +423,7 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
         }
         if (b0 + tid < p.B) s_place[b0 + tid] = before;
     }
-    const int dealt = chunk_dealt(p, least, most, all, items, longest, (int)gridDim.x);
+    dealt = chunk_dealt(p, least, most, all, items, longest, (int)gridDim.x);
     if (tid < p.phases) p.plan[tid * gridDim.x + blockIdx.x].at = -1;
     __syncthreads();
     // A warp to a phase: its stretch of this CTA.
@@ -439,6 +477,7 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
     }
     fence_proxy_async_smem();  // the sums' place is K's from here on
     __syncthreads();
+    }
     pdl_launch_dependents();  // the sums of parts: their CTAs wait where there is room for them
     const uint32_t tmem_base = *tmem_slot;
     const uint32_t tmem_s = tmem_base, tmem_o = tmem_base + 128;
@@ -456,7 +495,13 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
         // =============== one lane moves the tiles ===================================================
         if (elect_one()) {
             ChunkCursor kc;  // next K tile
-            kc.start(p, s_stretch, dealt);
+            if constexpr (CLUSTER) {
+                kc.u = mine;
+                kc.t = 0;
+                kc.valid = mine.n_tiles > 0;
+            } else {
+                kc.start(p, s_stretch, dealt);
+            }
             uint32_t gk = 0, gv = 0, nu = 0, nq = 0;  // copies issued; pieces posted, their Q tiles asked for
             auto post = [&](bool more) {
                 ChunkUnit &u = ring[nu % CH_RING];
@@ -527,7 +572,8 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
                 const int stage = (int)(gk % CH_STAGES);
                 load_tile(sK + stage * CH_KV_BYTES, maps.k, &bar_k[stage], kp, kc.u.hkv);
                 const bool ends = kc.last_of_unit();
-                kc.advance(p, s_stretch);
+                if constexpr (CLUSTER) kc.valid = ++kc.t < mine.n_tiles;
+                else kc.advance(p, s_stretch);
                 ++gk;
                 if (ends) post(kc.valid);
                 if (kc.valid) look_up(kp, kc.u, kc.t);
@@ -810,7 +856,7 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
                 const float inv = it.slot >= 0 ? 1.f : (l_run > 0.f ? 1.f / l_run : (l_run == l_run ? 0.f : l_run));
                 const long long part = (long long)it.slot * p.part_rows + row;
                 uint4 *dst = reinterpret_cast<uint4 *>(p.out + (((long long)it.b * p.T + it.t0 + tok) * p.Hq + it.hkv * p.G + head) * NCKV_D);
-                if (it.slot >= 0 && live) *reinterpret_cast<float2 *>(p.part_ml + part * 2) = make_float2(m_used, l_run);
+                if (it.slot >= 0 && live) (CLUSTER ? s_part_ml + row : reinterpret_cast<float2 *>(p.part_ml) + part)[0] = make_float2(m_used, l_run);
 #pragma unroll
                 for (int ch = 0; ch < NCKV_D / 32; ++ch) {
                     float c[32];
@@ -821,7 +867,11 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
 #pragma unroll
                             for (int i = 0; i < 32; ++i) c[i] += chunk_not_finite(p, it, pos, ch * 32 + i);
                         }
-                        if (it.slot >= 0) {
+                        if constexpr (CLUSTER) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                *reinterpret_cast<float4 *>(s_part + row * CH_PITCH + ch * 32 + i * 4) = make_float4(c[4 * i], c[4 * i + 1], c[4 * i + 2], c[4 * i + 3]);
+                        } else if (it.slot >= 0) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 uint32_t w[8];
@@ -854,6 +904,45 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
     tc_fence_before();
     __syncthreads();
     if (warp == 0) tmem_dealloc(tmem_base, CH_TMEM_COLS);
+    if constexpr (CLUSTER) {  // rows rank, rank + ctas, ...: the parts in the order of the keys, as in chunk_finish_kernel
+        const int ctas = (int)cluster_ctas(), rank = (int)cluster_rank(), rows = min(p.tile_tokens, mine.n) * p.G;
+        cluster_sync();
+        for (int row = rank + ctas * warp; row < rows; row += ctas * (CH_THREADS / 32)) {
+            float2 ml[8];
+            float m = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                ml[i] = make_float2(-INFINITY, 0.f);
+                if (i >= ctas) break;
+                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml[i].x), "=f"(ml[i].y) : "r"(smem_of_rank(s_part_ml + row, (uint32_t)i)) : "memory");
+                m = fmaxf(m, ml[i].x);
+            }
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            float l = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (i >= ctas) break;
+                if (ml[i].x == -INFINITY && ml[i].y == 0.f) continue;  // this row sees none of the part's keys
+                float4 x;
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+                             : "r"(smem_of_rank(s_part + row * CH_PITCH + lane * 4, (uint32_t)i))
+                             : "memory");
+                const float w = exp2f(ml[i].x - m);
+                l += w * ml[i].y;
+                o.x += w * x.x;
+                o.y += w * x.y;
+                o.z += w * x.z;
+                o.w += w * x.w;
+            }
+            const int tok = row / p.G, head = mine.hkv * p.G + row - tok * p.G;
+            const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+            reinterpret_cast<uint2 *>(p.out + (((long long)mine.b * p.T + tok) * p.Hq + head) * NCKV_D)[lane] =
+                make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+        }
+        __syncwarp();
+        cluster_sync();  // the others may still be reading
+    }
 }
 
 // Adds up the parts of a tile of queries whose keys were cut: O = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s.  Block (CTA, rows, phase) looks at
@@ -929,9 +1018,25 @@ static_assert(CH_RING * sizeof(ChunkUnit) >= 30 * 4, "the sums over the rows lie
 // How a launch of these sizes is cut: what of it doesn't depend on the rows' lengths.
 struct ChunkShape {
     int G, tile_tokens, n_qtiles, grid, phases, phase_pairs, part_rows;
+    int ctas;  // of a cluster; 0: no clusters
     long long n_items;
     size_t plan_bytes;
 };
+// CTAs to a pair (0: stretches) where rows have one tile of queries: as many as the chip has room for at once (two per SM, some lost between
+// clusters of 4 and 8), if a CTA's key tiles are then few and not many more than a stretch would have.  Lengths aren't known here, a full table is
+// taken for them.  us as stretches / clusters of 2 / 4 / 8, 6 + 6 heads, 4 tokens: 4 rows of up to 500 keys 11.8 / 9.3 / 9.0 / 8.6, 8 12.8 / 10.2 / 9.5 / 16.4,
+// 24 18.8 / 11.4 / 22.6 / 39.3; 4 rows of 4000 20.6 / 35.2 / 22.5 / 17.7, 2 of 8000 19.7 / 58.4 / 34.9 / 23.0; 16 rows of 4000, 16 + 4 heads 38.5 / 36.1 / 27.7 /
+// 36.6.  With 128 query rows stretches leave much larger partial sums: 4 x 32 tokens behind 8000, 16 + 4 heads 37.6 / 60.9 / 37.9 / 29.2.
+constexpr int CH_SHARE = 16;
+static int chunk_cluster(long long pairs, long long key_tiles, int part_rows) {
+    const long long room = 2LL * sm_count(), stretch = pairs * key_tiles / room;
+    for (int ctas = 8; ctas >= 1; ctas /= 2) {
+        if (pairs * ctas > (ctas > 2 ? room * 9 / 10 : room)) continue;
+        const long long share = (key_tiles + ctas - 1) / ctas;
+        return share <= CH_SHARE && share <= stretch + (part_rows <= 32 ? 8 : 20) ? ctas : 0;
+    }
+    return 0;
+}
 static ChunkShape chunk_shape(int B, int T, int Hq, int Hkv, long long capacity, long long window_left) {
     ChunkShape s;
     s.G = Hq / Hkv;
@@ -954,6 +1059,11 @@ static ChunkShape chunk_shape(int B, int T, int Hq, int Hkv, long long capacity,
     s.phase_pairs = (int)((pairs + s.phases - 1) / s.phases);
     s.phases = (int)((pairs + s.phase_pairs - 1) / s.phase_pairs);
     if (s.grid == 1) s.phases = 0;
+    s.ctas = s.n_qtiles == 1 && s.grid > 1 ? chunk_cluster(pairs, (keys + CH_N - 1) / CH_N, s.part_rows) : 0;
+    if (s.ctas) {
+        s.grid = (int)pairs * s.ctas;
+        s.phases = 0;
+    }
     s.plan_bytes = ((size_t)s.phases * s.grid * sizeof(ChunkPlan) + 255) / 256 * 256;
     return s;
 }
@@ -1074,11 +1184,13 @@ extern "C" int nckv_prefill_attn_paged(const void *q, const void *k_pool, const 
         p.group_pairs = (int)g;
     }
     const size_t smem = chunk_smem_bytes(s.part_rows);
+    const int ctas = s.ctas;
     static bool attr_set[64] = {false};
     int dev = 0;
     NCKV_CUDA_CHECK(cudaGetDevice(&dev));
     if (dev >= 64 || !attr_set[dev]) {
-        NCKV_CUDA_CHECK(cudaFuncSetAttribute(chunk_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)chunk_smem_bytes(CH_M)));
+        NCKV_CUDA_CHECK(cudaFuncSetAttribute(chunk_attn_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)chunk_smem_bytes(CH_M)));
+        NCKV_CUDA_CHECK(cudaFuncSetAttribute(chunk_attn_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)chunk_smem_bytes(CH_M)));
         if (dev < 64) attr_set[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
@@ -1086,12 +1198,19 @@ extern "C" int nckv_prefill_attn_paged(const void *q, const void *k_pool, const 
     cfg.blockDim = dim3(CH_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)ctas;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    NCKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, chunk_attn_kernel, maps, p));
+    cfg.numAttrs = ctas ? 2 : 1;
+    if (ctas) {
+        NCKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, chunk_attn_kernel<true>, maps, p));
+        return NCKV_OK;
+    }
+    NCKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, chunk_attn_kernel<false>, maps, p));
     if (s.phases) {
         // few rows: all of a block's warps to one, over the parts
         const bool wide = s.part_rows <= 16;
