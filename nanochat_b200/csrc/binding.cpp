@@ -134,6 +134,90 @@ std::optional<Tensor> kv_attention(const Tensor &q, const Tensor &k, const Tenso
     return y;
 }
 
+// Attention of several new tokens per row over page pools: nckv_prefill_attn_paged.
+std::optional<Tensor> prefill_attention_paged(const Tensor &q, const Tensor &k_pool, const Tensor &v_pool, const Tensor &block_table, const Tensor &seqlens,
+                                              const std::optional<Tensor> &new_tokens, int64_t window_left) {
+    if (!q.is_cuda() || q.dim() != 4 || k_pool.dim() != 4 || v_pool.dim() != 4 || block_table.dim() != 2) return std::nullopt;
+    const c10::Device dev = q.device();
+    for (const Tensor *t : {&q, &k_pool, &v_pool})
+        if (!bf16_on(*t, dev)) return std::nullopt;
+    const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), Hkv = k_pool.size(2);
+    auto ints = [&](const Tensor &t) { return t.scalar_type() == at::kInt && t.device() == dev && t.is_contiguous(); };
+    if (q.numel() == 0 || q.numel() / D > INT_MAX || !q.is_contiguous() || q.size(3) != D || Hkv <= 0 || Hq % Hkv || k_pool.sizes() != v_pool.sizes() ||
+        k_pool.strides() != v_pool.strides() || k_pool.size(3) != D || k_pool.stride(3) != 1 || k_pool.stride(2) != D ||
+        k_pool.size(1) % nckv_paged_tile_tokens() || k_pool.size(0) > INT_MAX || k_pool.size(1) > INT_MAX || !ints(block_table) ||
+        block_table.size(0) != B || block_table.size(1) > INT_MAX || !ints(seqlens) || seqlens.dim() != 1 || seqlens.numel() != B ||
+        (new_tokens && (!ints(*new_tokens) || new_tokens->dim() != 1 || new_tokens->numel() != B)) || window_left < -1 || window_left > (1 << 30))
+        return std::nullopt;
+    const auto on = launch_on(dev, 1, 1, 1);
+    if (!on) return std::nullopt;
+
+    const pybind11::gil_scoped_release unlocked;
+    const c10::cuda::CUDAGuard guard(dev);
+    const int page = (int)k_pool.size(1), pages = (int)block_table.size(1);
+    const size_t need = nckv_prefill_attn_paged_workspace_bytes((int)B, (int)T, (int)Hq, (int)Hkv, page, pages, (int)window_left);
+    Tensor out = at::empty(q.sizes(), q.options()), scratch;
+    if (need) scratch = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
+    if (nckv_prefill_attn_paged(q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), static_cast<const int32_t *>(block_table.data_ptr()),
+                                static_cast<const int32_t *>(seqlens.data_ptr()), new_tokens ? static_cast<const int32_t *>(new_tokens->data_ptr()) : nullptr,
+                                out.data_ptr(), (int)B, (int)T, (int)Hq, (int)Hkv, (int)D, page, pages, (int)k_pool.size(0), k_pool.stride(0), k_pool.stride(1),
+                                (int)window_left, need ? scratch.data_ptr() : nullptr, need, static_cast<int32_t *>(on->ws.data_ptr()), on->stream) < 0)
+        return std::nullopt;
+    return out;
+}
+
+// Distance between the rows of (..., C) activations with packed channels, or -1.
+int64_t rows_apart(const Tensor &t) {
+    const int64_t C = t.size(-1);
+    if (t.stride(-1) != 1 || (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15)) return -1;
+    int64_t stride = C, inner = 0;  // of the innermost dimension that has a distance; the distance that the next one out has to have
+    bool found = false;
+    for (int64_t i = t.dim() - 2; i >= 0; --i) {
+        if (t.size(i) == 1) continue;
+        if (!found) stride = t.stride(i);
+        else if (t.stride(i) != inner) return -1;
+        found = true;
+        inner = t.stride(i) * t.size(i);
+    }
+    return stride >= C && stride % 8 == 0 ? stride : -1;
+}
+
+// What requests' low-rank adapters add to a shared product: nckv_adapters, into y or beside it.
+std::optional<Tensor> add_adapters(const Tensor &y, const Tensor &x, const Tensor &down, const Tensor &up, const Tensor &slots, const Tensor &scales,
+                                   bool in_place) {
+    if (!y.is_cuda() || y.dim() < 2 || x.dim() != y.dim() || down.dim() != 3 || up.dim() != 3 || slots.dim() != 1 || scales.dim() != 1) return std::nullopt;
+    const c10::Device dev = y.device();
+    for (const Tensor *t : {&y, &x, &down, &up})
+        if (!bf16_on(*t, dev)) return std::nullopt;
+    if (at::GradMode::is_enabled() && (y.requires_grad() || x.requires_grad() || down.requires_grad() || up.requires_grad() || scales.requires_grad()))
+        return std::nullopt;
+    const int64_t S = down.size(0), R = down.size(1), K = down.size(2), N = up.size(1), B = slots.numel();
+    if (y.numel() == 0 || x.size(-1) != K || y.size(-1) != N || up.size(0) != S || up.size(2) != R || !down.is_contiguous() || !up.is_contiguous() ||
+        slots.scalar_type() != at::kInt || slots.device() != dev || !slots.is_contiguous() || scales.scalar_type() != at::kFloat || scales.device() != dev ||
+        scales.numel() != S || !scales.is_contiguous() || ((reinterpret_cast<uintptr_t>(down.data_ptr()) | reinterpret_cast<uintptr_t>(up.data_ptr())) & 15))
+        return std::nullopt;
+    for (int64_t i = 0; i < y.dim() - 1; ++i)
+        if (x.size(i) != y.size(i)) return std::nullopt;
+    const int64_t rows = y.numel() / N;
+    if (B == 0 || rows % B || rows > INT_MAX || K > INT_MAX || N > INT_MAX || S > INT_MAX || R > INT_MAX) return std::nullopt;
+    const int64_t y_stride = rows_apart(y), x_stride = rows_apart(x);
+    if (y_stride < 0 || x_stride < 0) return std::nullopt;
+    const auto on = launch_on(dev, 1, 1, 1);
+    if (!on) return std::nullopt;
+
+    const pybind11::gil_scoped_release unlocked;
+    const c10::cuda::CUDAGuard guard(dev);
+    const int b = (int)B, t = (int)(rows / B), k = (int)K, n = (int)N, r = (int)R, s = (int)S;
+    const size_t need = nckv_adapters_workspace_bytes(b, t, k, n, r, s);
+    Tensor out = in_place ? y : at::empty(y.sizes(), y.options()), scratch;
+    if (need) scratch = at::empty({(int64_t)need}, y.options().dtype(at::kByte));
+    if (nckv_adapters(y.data_ptr(), y_stride, x.data_ptr(), x_stride, down.data_ptr(), up.data_ptr(), static_cast<const int32_t *>(slots.data_ptr()),
+                      static_cast<const float *>(scales.data_ptr()), out.data_ptr(), in_place ? y_stride : N, b, t, k, n, r, s,
+                      need ? scratch.data_ptr() : nullptr, need, static_cast<int32_t *>(on->ws.data_ptr()), on->stream) < 0)
+        return std::nullopt;
+    return out;
+}
+
 // Rows of the trunk's elementwise kernels: contiguous bf16 on one device.
 bool row_tensor(const Tensor &t, const Tensor &like) {
     return bf16_on(t, like.device()) && t.is_contiguous() && t.sizes() == like.sizes();
@@ -215,6 +299,8 @@ std::optional<Tensor> glue_relu_sq(const Tensor &h) {
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("set_workspace", &set_workspace);
     m.def("kv_attention", &kv_attention);
+    m.def("prefill_attention_paged", &prefill_attention_paged);
+    m.def("add_adapters", &add_adapters);
     m.def("glue_mix_norm", &glue_mix_norm);
     m.def("glue_mix_norm_at", &glue_mix_norm_at);
     m.def("glue_relu_sq", &glue_relu_sq);

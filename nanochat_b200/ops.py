@@ -744,6 +744,9 @@ def prefill_attention_paged(q, k_pool, v_pool, block_table, cache_seqlens, new_t
     """``prefill_attention`` over paged storage that holds the new keys already: q (B, T, Hq, D), row b's queries at
     positions ``cache_seqlens[b] + t``.  With ``new_tokens`` (int32 per row) only the first ``new_tokens[b]`` of a row's T
     slots hold a token; the output is zero in the others."""
+    done = _lib.native.prefill_attention_paged(q, k_pool, v_pool, block_table, cache_seqlens, new_tokens, window_left)
+    if done is not None:
+        return done
     name = "prefill_attn_paged"
     _require_cuda(name, q, k_pool, v_pool, block_table, cache_seqlens, new_tokens)
     _require_bf16(name, q, k_pool, v_pool)
@@ -998,6 +1001,9 @@ def add_adapters(y, x, down, up, slots, scales):
     adapter adds to the output of a projection that all of them share.  x (..., K) and y (..., N) bf16 hold the rows of ``slots.numel()``
     requests one after the other, as many for each; down (S, R, K), up (S, N, R) bf16; scales (S,) float32; slots int32.  K, N and R are
     multiples of 8, R at most 128.  Sums in float32, rounded once."""
+    done = _lib.native.add_adapters(y, x, down, up, slots, scales, False)
+    if done is not None:
+        return done
     out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
     _adapters("add_adapters", y, x, down, up, slots, scales, out)
     return out
@@ -1005,6 +1011,8 @@ def add_adapters(y, x, down, up, slots, scales):
 
 def add_adapters_(y, x, down, up, slots, scales):
     """The same into y, which may be a column slice of a wider product; rows without an adapter are not touched.  Returns y."""
+    if _lib.native.add_adapters(y, x, down, up, slots, scales, True) is not None:
+        return y
     _adapters("add_adapters_", y, x, down, up, slots, scales, None)
     return y
 

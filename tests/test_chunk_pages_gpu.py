@@ -113,6 +113,29 @@ def test_many_rows_and_uniform_prompts():
     check(ops.prefill_attention_paged(*args), *args, -1)
 
 
+@pytest.mark.parametrize("B,T,Hq,Hkv,lens,window,counts", [
+    (48, 5, 16, 4, [(97 * i) % 1500 for i in range(48)], -1, False),         # equal stretches, several pieces each
+    (48, 5, 16, 4, [(97 * i) % 1500 for i in range(48)], 300, True),
+    (24, 96, 16, 4, [(211 * i) % 900 for i in range(24)], 128, True),        # dealt row by row
+    (6, 300, 6, 6, [1000 + i for i in range(6)], -1, False),                 # dealt in the order of like rows
+    (3, 70, 16, 2, [9000, 10, 4000], -1, False),                             # cut, several tiles of queries
+    (2, 40, 16, 4, [8100, 8000], -1, False),
+    (70, 2, 2, 2, [i for i in range(70)], -1, True),                         # a CTA to a pair
+    (12, 16, 8, 8, [400] * 12, 63, False),                                   # clusters of 2
+])
+def test_all_ways_of_sharing_the_work(B, T, Hq, Hkv, lens, window, counts):
+    from nanochat_b200 import ops
+    new = [(5 * i + 3) % (T + 1) for i in range(B)] if counts else None
+    args = make(B, T, Hq, Hkv, 48, lens, seed=B + T, new=new)
+    got = ops.prefill_attention_paged(*args[:5], args[5] if counts else None, window)
+    assert ops.read_status(DEV) == 0
+    check(got, *args, window)
+    again = ops.prefill_attention_paged(*args[:5], args[5] if counts else None, window)
+    assert torch.equal(got.view(torch.int16), again.view(torch.int16))
+    for b in range(B):
+        assert not got[b, int(args[5][b]):].any()
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 def test_values_that_are_not_finite_reach_only_who_sees_them(bad):
     from nanochat_b200 import ops
