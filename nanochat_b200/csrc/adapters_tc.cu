@@ -21,7 +21,7 @@ constexpr int AT_THREADS = 192;             // copies, products, four warps for 
 constexpr int AT_UP_THREADS = 64 + 2 * 128;  // two groups of four take steps in turn
 constexpr int AT_ACCS = 4;                   // accumulators of adapter_tile_up
 constexpr int AT_X_BYTES = AT_M * AT_K * 2;
-constexpr int AT_DOWN_STAGES = 4, AT_MAX_CLUSTER = 8;
+constexpr int AT_DOWN_STAGES = 6, AT_MAX_CLUSTER = 8;
 
 struct AdapterTile {
     AdapterParams a;
@@ -94,7 +94,8 @@ adapter_tile_down(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         *abort_flag = 1;
         atomicOr(p.status, (int)NCKV_ST_TIMEOUT);
     };
-    const int steps = (p.K + AT_K - 1) / AT_K, k_lo = steps * rank / ctas, n = steps * (rank + 1) / ctas - k_lo;  // n > 0: at most as many CTAs as steps
+    // every ctas-th step: the cluster reads a row's channels side by side (n > 0: at most as many CTAs as steps)
+    const int steps = (p.K + AT_K - 1) / AT_K, n = (steps - rank + ctas - 1) / ctas;
     if (*abort_flag) {
         if (tid == 0) timed_out();
     } else if (warp == 0) {
@@ -107,8 +108,8 @@ adapter_tile_down(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 if (!ok) break;
                 uint8_t *at = smem + s * stage_bytes;
                 mbar_arrive_expect_tx(&bar_full[s], stage_bytes);
-                tma_load_3d(at, &map_x, &bar_full[s], (k_lo + i) * AT_K, t0, b);
-                tma_load_3d(at + AT_X_BYTES, &map_down, &bar_full[s], (k_lo + i) * AT_K, 0, slot);
+                tma_load_3d(at, &map_x, &bar_full[s], (i * ctas + rank) * AT_K, t0, b);
+                tma_load_3d(at + AT_X_BYTES, &map_down, &bar_full[s], (i * ctas + rank) * AT_K, 0, slot);
                 ++issued;
             }
             if (!ok) timed_out();
@@ -420,7 +421,7 @@ int adapters_tc(const AdapterParams &a, cudaStream_t stream) {
         return NCKV_E_UNSUPPORTED;
     }
     int ctas = 1;  // of a cluster: a power of two that a tile's rows and channels can be shared by
-    while (ctas < AT_MAX_CLUSTER && 2 * ctas * tiles <= 2 * sms && 2 * ctas <= (a.K + AT_K - 1) / AT_K) ctas *= 2;
+    while (ctas < AT_MAX_CLUSTER && 2 * ctas * tiles <= sms && 2 * ctas <= (a.K + AT_K - 1) / AT_K) ctas *= 2;  // (two to an SM: a third were on it at a time)
     q.stages = 8;
     while (q.stages > 4 && adapter_up_smem(q.RP, a.R, q.stages) > 220 * 1024) --q.stages;
     const size_t down_smem = adapter_down_smem(q.RP), up_smem = adapter_up_smem(q.RP, a.R, q.stages);
