@@ -909,31 +909,32 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
         cluster_sync();
         for (int row = rank + ctas * warp; row < rows; row += ctas * (CH_THREADS / 32)) {
             float2 ml[8];
-            float m = -INFINITY;
+            float4 x[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 8; ++i) {  // all of them on their way at once
                 ml[i] = make_float2(-INFINITY, 0.f);
-                if (i >= ctas) break;
-                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml[i].x), "=f"(ml[i].y) : "r"(smem_of_rank(s_part_ml + row, (uint32_t)i)) : "memory");
-                m = fmaxf(m, ml[i].x);
+                x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i < ctas) {
+                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml[i].x), "=f"(ml[i].y) : "r"(smem_of_rank(s_part_ml + row, (uint32_t)i)) : "memory");
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                 : "=f"(x[i].x), "=f"(x[i].y), "=f"(x[i].z), "=f"(x[i].w)
+                                 : "r"(smem_of_rank(s_part + row * CH_PITCH + lane * 4, (uint32_t)i))
+                                 : "memory");
+                }
             }
+            float m = -INFINITY, l = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, ml[i].x);
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            float l = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                if (i >= ctas) break;
-                if (ml[i].x == -INFINITY && ml[i].y == 0.f) continue;  // this row sees none of the part's keys
-                float4 x;
-                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                             : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
-                             : "r"(smem_of_rank(s_part + row * CH_PITCH + lane * 4, (uint32_t)i))
-                             : "memory");
+                if (ml[i].x == -INFINITY && ml[i].y == 0.f) continue;  // this row sees none of the part's keys; what lies there is nothing
                 const float w = exp2f(ml[i].x - m);
                 l += w * ml[i].y;
-                o.x += w * x.x;
-                o.y += w * x.y;
-                o.z += w * x.z;
-                o.w += w * x.w;
+                o.x += w * x[i].x;
+                o.y += w * x[i].y;
+                o.z += w * x[i].z;
+                o.w += w * x[i].w;
             }
             const int tok = row / p.G, head = mine.hkv * p.G + row - tok * p.G;
             const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
