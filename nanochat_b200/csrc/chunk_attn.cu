@@ -48,8 +48,9 @@ struct ChunkMaps {
     CUtensorMap q, k[4], v[4];  // k, v: boxes of 16, 32, 48 and 64 keys of 64 channels
 };
 
-struct ChunkPlan {  // a CTA's stretch of a phase: its first key tile (-1: none), how far into which tile of queries that is, and the whole tile's key tiles
+struct alignas(16) ChunkPlan {  // a CTA's stretch of a phase: its first key tile (-1: none), how far into which tile of queries that is, and the whole tile's key tiles
     int at, off, count, b, hkv, t0, begin, each;  // the phase begins at `begin` and is cut every `each`
+    int n, none[3];                               // new tokens of the row
 };
 
 struct ChunkParams {
@@ -471,7 +472,7 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
             st.off = off;
             if (lane == 0) {
                 s_stretch[warp] = st;
-                p.plan[warp * gridDim.x + blockIdx.x] = ChunkPlan{st.at, off, count, row, st.hkv, st.qt * p.tile_tokens, lo, each};
+                p.plan[warp * gridDim.x + blockIdx.x] = ChunkPlan{st.at, off, count, row, st.hkv, st.qt * p.tile_tokens, lo, each, r.n, {0, 0, 0}};
             }
         }
     }
@@ -960,7 +961,7 @@ __global__ void __launch_bounds__(256) chunk_finish_kernel(const __grid_constant
     if (cut.at < 0 || cut.off == 0) return;
     const int from = cut.at - cut.off - cut.begin, first = from / cut.each, last = (from + cut.count - 1) / cut.each, parts = last - first + 1;
     if (c != first + 1) return;
-    const int n = chunk_row(p, cut.b).n, rows = min(p.tile_tokens, n - cut.t0) * p.G;
+    const int rows = min(p.tile_tokens, cut.n - cut.t0) * p.G;
     const long long slot0 = ((long long)phase * grid + first) * 2;
     const bool second = first * cut.each < from;  // the first part is not the first piece of its stretch
     auto part_of = [&](int i, int row) -> long long { return (slot0 + 2 * i + (i == 0 && second)) * p.part_rows + row; };
@@ -970,24 +971,39 @@ __global__ void __launch_bounds__(256) chunk_finish_kernel(const __grid_constant
     for (int k = 0; k < EACH; ++k) {
         const int row = row0 + k * STEP;
         if (row >= rows) return;  // uniform over the warps of a row
+        // this warp's first two parts are asked for beside all parts' maxima
+        constexpr int AHEAD = 2;
+        float2 ml[AHEAD];
+        float4 x[AHEAD];
+#pragma unroll
+        for (int k2 = 0; k2 < AHEAD; ++k2) {
+            const int i = mine + k2 * WARPS;
+            ml[k2] = make_float2(-INFINITY, 0.f);
+            x[k2] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (i < parts) {
+                ml[k2] = *reinterpret_cast<const float2 *>(p.part_ml + part_of(i, row) * 2);
+                x[k2] = reinterpret_cast<const float4 *>(p.part_o + part_of(i, row) * NCKV_D)[lane];
+            }
+        }
         float m = -INFINITY, l = 0.f;
         for (int i = lane; i < parts; i += 32) m = fmaxf(m, p.part_ml[part_of(i, row) * 2]);
 #pragma unroll
         for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](float2 part, float4 v) {
+            if (part.x == -INFINITY && part.y == 0.f) return;  // this row sees none of the part's keys
+            const float w = exp2f(part.x - m);
+            l += w * part.y;
+            o.x += w * v.x;
+            o.y += w * v.y;
+            o.z += w * v.z;
+            o.w += w * v.w;
+        };
+#pragma unroll
+        for (int k2 = 0; k2 < AHEAD; ++k2) add(ml[k2], x[k2]);
 #pragma unroll 4
-        for (int i = mine; i < parts; i += WARPS) {
-            const long long at = part_of(i, row);
-            const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + at * 2);
-            const float4 x = reinterpret_cast<const float4 *>(p.part_o + at * NCKV_D)[lane];
-            if (ml.x == -INFINITY && ml.y == 0.f) continue;  // this row sees none of the part's keys
-            const float w = exp2f(ml.x - m);
-            l += w * ml.y;
-            o.x += w * x.x;
-            o.y += w * x.y;
-            o.z += w * x.z;
-            o.w += w * x.w;
-        }
+        for (int i = mine + AHEAD * WARPS; i < parts; i += WARPS)
+            add(*reinterpret_cast<const float2 *>(p.part_ml + part_of(i, row) * 2), reinterpret_cast<const float4 *>(p.part_o + part_of(i, row) * NCKV_D)[lane]);
         if constexpr (WARPS > 1) {
             s_o[warp][lane] = o;
             if (lane == 0) s_l[warp] = l;
