@@ -39,7 +39,7 @@ constexpr int CH_KV_BYTES = CH_N * NCKV_D * 2;
 constexpr int CH_TMEM_COLS = 256;  // S / P buffers [0, 64), [64, 128); O [128, 256)
 constexpr int CH_PHASES = 4;       // most groups of pairs that are cut one after the other
 constexpr int CH_MIN_TILES = 1;    // shortest stretch of a CTA
-constexpr int CH_ROWS = 8192;      // most rows of a launch: 64 KB of shared memory that the keys come to later
+constexpr int CH_ROWS = 4096;      // most rows of a launch: 48 KB of shared memory that the keys come to later
 constexpr int CH_RING = 8;         // pieces of work that the copying thread can be ahead with: it is four at most (five stages, pieces of one tile)
 constexpr int CH_PITCH = NCKV_D + 4;  // floats of a row where a cluster's parts meet
 constexpr long long CH_PART_BYTES = 160LL << 20, CH_PHASE_BYTES = 48LL << 20;
@@ -53,11 +53,17 @@ struct alignas(16) ChunkPlan {  // a CTA's stretch of a phase: its first key til
     int n, none[3];                               // new tokens of the row
 };
 
+struct alignas(16) ChunkDeal {  // an uncut tile of queries: row (-1: nothing), kv head + Hkv * number of the tile, the row's lengths
+    int b, local, L, n;
+};
+
 struct ChunkParams {
     const int32_t *table, *seqlens, *new_tokens;  // new_tokens may be null: T for every row
     const __nv_bfloat16 *v_pool;
     __nv_bfloat16 *out;
-    ChunkPlan *plan; // (phases, CTAs): how the stretches were cut
+    ChunkPlan *plan;    // (phases, CTAs): how the stretches were cut
+    ChunkDeal *deals;   // (CTAs, rounds): what was dealt
+    int rounds;
     float *part_ml;  // (slots, part_rows, 2): maximum and sum
     float *part_o;   // (slots, part_rows, 128), not divided by the sum
     int32_t *status;
@@ -114,20 +120,23 @@ struct ChunkCursor {
     int t;    // key tile inside the piece
     int seq;  // number of the piece among the CTA's
     bool valid;
-    int phase;  // -1: dealt, -2: dealt row by row
+    int phase;  // -1: dealt
     int at;     // next key tile of the stretch, or next round of the deal
-    int begin, end, qt, off;  // (dealt row by row: row `end`, and the tiles of queries before it)
+    int begin, end, qt, off;
     ChunkSpan span;
+    // Looked up ahead of need: a row's lengths, or an entry of the deal, take longer than a key tile.
+    ChunkRow next_row;
+    ChunkDeal next_deal;
 
     __device__ __forceinline__ void item(const ChunkParams &p) {
         u.t0 = qt * p.tile_tokens;
         span = chunk_span(p, ChunkRow{u.L, u.n}, u.t0);
     }
-    __device__ __forceinline__ void row(const ChunkParams &p, int b) {
-        const ChunkRow r = chunk_row(p, b);
+    __device__ __forceinline__ void row(const ChunkParams &p, int b, const ChunkRow &r) {
         u.b = b;
         u.L = r.L;
         u.n = r.n;
+        next_row = chunk_row(p, min(b + 1, p.B - 1));
     }
     __device__ __forceinline__ bool enter(const ChunkParams &p, const ChunkStretch *stretches) {  // the next phase with something in it
         for (; phase < p.phases; ++phase) {
@@ -135,7 +144,7 @@ struct ChunkCursor {
             if (s.at >= s.end) continue;
             at = begin = s.at;
             end = s.end;
-            row(p, s.b);
+            row(p, s.b, chunk_row(p, s.b));
             u.hkv = s.hkv;
             qt = s.qt;
             off = s.off;
@@ -144,19 +153,20 @@ struct ChunkCursor {
         }
         return false;
     }
-    __device__ __forceinline__ void start(const ChunkParams &p, const ChunkStretch *stretches, int dealt) {
+    // `deals`: rounds that were dealt to this CTA, -1: stretches
+    __device__ __forceinline__ void start(const ChunkParams &p, const ChunkStretch *stretches, int deals) {
         seq = -1;
+        at = begin = 0;
+        end = deals;
+        phase = deals < 0 ? 0 : -1;
         valid = true;
-        at = end = begin = 0;
-        phase = -dealt;
-        if (!dealt) valid = enter(p, stretches);
-        if (dealt == 2) row(p, 0);
+        if (deals < 0) valid = enter(p, stretches);
+        else if (deals > 0) next_deal = p.deals[(long long)blockIdx.x * p.rounds];
         if (valid) load(p, stretches);
     }
     __device__ __forceinline__ void load(const ChunkParams &p, const ChunkStretch *stretches) {
         t = 0;
         ++seq;
-        const int grid = (int)gridDim.x, c = (int)blockIdx.x;
         if (phase >= 0) {
             if (at >= end) {
                 ++phase;
@@ -169,7 +179,7 @@ struct ChunkCursor {
                         qt = 0;
                         if (++u.hkv == p.Hkv) {
                             u.hkv = 0;
-                            do row(p, u.b + 1);
+                            do row(p, u.b + 1, next_row);
                             while (u.n == 0);
                         }
                     }
@@ -180,47 +190,30 @@ struct ChunkCursor {
             u.kv_hi = span.kv_hi;
             u.n_tiles = min(span.count - off, end - at);
             u.tile0 = span.first + off;
-            u.slot = u.n_tiles == span.count ? -1 : (phase * grid + c) * 2 + (at != begin);
+            u.slot = u.n_tiles == span.count ? -1 : (phase * (int)gridDim.x + (int)blockIdx.x) * 2 + (at != begin);
             off += u.n_tiles;
             at += u.n_tiles;
             return;
         }
-        const int pairs = p.B * p.Hkv, per_group = p.group_pairs * p.n_qtiles;
-        for (;; ++at) {
-            const long long idx = (long long)at * grid + ((at & 1) ? grid - 1 - c : c);  // dealt back and forth
-            if (idx >= (long long)pairs * p.n_qtiles) {  // none in this round, then none later
+        for (;;) {
+            if (at >= end) {
                 valid = false;
                 return;
             }
-            if (phase == -2) {
-                int tiles;  // of queries, of one kv head of the row
-                while (tiles = (u.n + p.tile_tokens - 1) / p.tile_tokens, idx >= begin + tiles * p.Hkv) {
-                    begin += tiles * p.Hkv;
-                    if (++end == p.B) {
-                        valid = false;
-                        return;
-                    }
-                    row(p, end);
-                }
-                const int local = (int)idx - begin;
-                qt = tiles - 1 - local / p.Hkv;
-                u.hkv = local % p.Hkv;
-            } else {
-                const int grp = min((int)idx / per_group, p.n_groups - 1), in_grp = (int)idx - grp * per_group;
-                const int grp_pairs = grp == p.n_groups - 1 ? pairs - grp * p.group_pairs : p.group_pairs;
-                const int pair = grp * p.group_pairs + in_grp % grp_pairs;
-                qt = p.n_qtiles - 1 - in_grp / grp_pairs;  // all pairs' longest tiles first
-                row(p, pair / p.Hkv);
-                if (qt * p.tile_tokens >= u.n) continue;
-                u.hkv = pair - u.b * p.Hkv;
-            }
+            const ChunkDeal d = next_deal;
+            if (++at < end) next_deal = p.deals[(long long)blockIdx.x * p.rounds + at];
+            if (d.b < 0) continue;
+            u.b = d.b;
+            u.L = d.L;
+            u.n = d.n;
+            qt = d.local / p.Hkv;
+            u.hkv = d.local - qt * p.Hkv;
             item(p);
             u.kv_lo = span.kv_lo;
             u.kv_hi = span.kv_hi;
             u.n_tiles = span.count;
             u.tile0 = span.first;
             u.slot = -1;
-            ++at;
             return;
         }
     }
@@ -292,7 +285,7 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     volatile int *s_poison = reinterpret_cast<volatile int *>(tmem_slot + 2);        // [4]: piece seq (seq & 3) had values that are not finite
     ChunkStretch *s_stretch = reinterpret_cast<ChunkStretch *>(tmem_slot + 6);       // [CH_PHASES]
-    int *s_sum = reinterpret_cast<int *>(ring);                                      // [5][6], before there are pieces
+    int *s_sum = reinterpret_cast<int *>(ring);                                      // [6][6], before there are pieces
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -319,7 +312,7 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
         tmem_relinquish();
     }
     pdl_wait_prior_grids();  // lengths and tables may come from the grid before
-    int dealt = 0;
+    int dealt = 0, deals = -1;
     bool any_idle = false;
     [[maybe_unused]] ChunkUnit mine;
     // where a cluster's parts meet: where K and V have been
@@ -354,8 +347,9 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
     tc_fence_after();
     } else {
     // ---- lengths: `width` lanes to a row -----------------------------------------------------------------
-    // s_tiles[b]: key tiles of row b's tiles of queries, per kv head; s_place[b]: key tiles before row b.  They lie where K and V come later.
-    int *s_tiles = reinterpret_cast<int *>(sK), *s_place = s_tiles + CH_ROWS;
+    // s_tiles[b]: key tiles of row b's tiles of queries, per kv head; s_place[b]: key tiles before row b; s_items[b]: tiles of queries, in all heads,
+    // then those before row b.  They lie where K and V come later.
+    int *s_tiles = reinterpret_cast<int *>(sK), *s_place = s_tiles + CH_ROWS, *s_items = s_place + CH_ROWS;
     int width = 1;
     while (width < 32 && width < p.n_qtiles) width *= 2;
     const int member = tid & (width - 1), groups = CH_THREADS / width;
@@ -379,7 +373,8 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
         for (int off = 1; off < width; off <<= 1) n += __shfl_xor_sync(mask, n, off);
         if (member == 0) {
             s_tiles[b] = n;
-            items += (r.n + p.tile_tokens - 1) / p.tile_tokens * p.Hkv;
+            s_items[b] = (r.n + p.tile_tokens - 1) / p.tile_tokens * p.Hkv;
+            items += s_items[b];
             least = min(least, n);
             most = max(most, n);
         }
@@ -405,28 +400,77 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
         least = min(least, s_sum[12 + w]);
         most = max(most, s_sum[18 + w]);
     }
-    int all = 0;  // key tiles before a chunk of rows, then of all
+    int all = 0, all_items = 0;  // key tiles and tiles of queries before a chunk of rows, then of all
     for (int b0 = 0; b0 < p.B; b0 += CH_THREADS) {
-        const int mine = b0 + tid < p.B ? s_tiles[b0 + tid] * p.Hkv : 0;
-        int before = mine;
+        const int mine = b0 + tid < p.B ? s_tiles[b0 + tid] * p.Hkv : 0, my_items = b0 + tid < p.B ? s_items[b0 + tid] : 0;
+        int before = mine, items_before = my_items;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, before, off);
-            if (lane >= off) before += v;
+            const int v = __shfl_up_sync(0xffffffffu, before, off), w = __shfl_up_sync(0xffffffffu, items_before, off);
+            if (lane >= off) {
+                before += v;
+                items_before += w;
+            }
         }
         if (b0) __syncthreads();  // the sums of the chunk before have been read
-        if (lane == 31) s_sum[24 + warp] = before;
+        if (lane == 31) {
+            s_sum[24 + warp] = before;
+            s_sum[30 + warp] = items_before;
+        }
         __syncthreads();
         before += all - mine;
+        items_before += all_items - my_items;
         for (int w = 0; w < CH_THREADS / 32; ++w) {
-            if (w < warp) before += s_sum[24 + w];
+            if (w < warp) {
+                before += s_sum[24 + w];
+                items_before += s_sum[30 + w];
+            }
             all += s_sum[24 + w];
+            all_items += s_sum[30 + w];
         }
-        if (b0 + tid < p.B) s_place[b0 + tid] = before;
+        if (b0 + tid < p.B) {
+            s_place[b0 + tid] = before;
+            s_items[b0 + tid] = items_before;
+        }
     }
     dealt = chunk_dealt(p, least, most, all, items, longest, (int)gridDim.x);
     if (tid < p.phases) p.plan[tid * gridDim.x + blockIdx.x].at = -1;
     __syncthreads();
+    if (dealt) {
+        // a thread to a round; dealt back and forth
+        const int pairs = p.B * p.Hkv, per_group = p.group_pairs * p.n_qtiles, limit = dealt == 2 ? items : pairs * p.n_qtiles;
+        const int grid = (int)gridDim.x, c = (int)blockIdx.x;
+        deals = limit / grid;
+        deals += ((deals & 1) ? grid - 1 - c : c) < limit - deals * grid;
+        for (int i = tid; i < deals; i += CH_THREADS) {
+            const int idx = i * grid + ((i & 1) ? grid - 1 - c : c);
+            ChunkDeal d;
+            if (dealt == 2) {
+                int lo = 0, hi = p.B - 1;  // the first row with tiles behind idx
+                while (lo < hi) {
+                    const int mid = (lo + hi) / 2;
+                    if (s_items[mid + 1] > idx) hi = mid;
+                    else lo = mid + 1;
+                }
+                d.b = lo;
+                const ChunkRow r = chunk_row(p, lo);
+                const int in_row = idx - s_items[lo], qt = (r.n + p.tile_tokens - 1) / p.tile_tokens - 1 - in_row / p.Hkv;  // longest first
+                d.local = qt * p.Hkv + in_row % p.Hkv;
+                d.L = r.L;
+                d.n = r.n;
+            } else {
+                const int grp = min(idx / per_group, p.n_groups - 1), in_grp = idx - grp * per_group;
+                const int grp_pairs = grp == p.n_groups - 1 ? pairs - grp * p.group_pairs : p.group_pairs;
+                const int pair = grp * p.group_pairs + in_grp % grp_pairs, qt = p.n_qtiles - 1 - in_grp / grp_pairs;  // all pairs' longest tiles first
+                const ChunkRow r = chunk_row(p, pair / p.Hkv);
+                d.b = qt * p.tile_tokens < r.n ? pair / p.Hkv : -1;
+                d.local = qt * p.Hkv + pair % p.Hkv;
+                d.L = r.L;
+                d.n = r.n;
+            }
+            p.deals[(long long)c * p.rounds + i] = d;
+        }
+    }
     // A warp to a phase: its stretch of this CTA.
     if (!dealt && warp < p.phases) {
         auto place = [&](int pair) {  // key tiles before a (row, kv head)
@@ -501,7 +545,7 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
                 kc.t = 0;
                 kc.valid = mine.n_tiles > 0;
             } else {
-                kc.start(p, s_stretch, dealt);
+                kc.start(p, s_stretch, deals);
             }
             uint32_t gk = 0, gv = 0, nu = 0, nq = 0;  // copies issued; pieces posted, their Q tiles asked for
             auto post = [&](bool more) {
@@ -1030,14 +1074,15 @@ static size_t chunk_smem_bytes(int part_rows) {
     return 2 * (part_rows <= CH_M / 2 ? 2 : 1) * chunk_q_half(part_rows) + (CH_STAGES + CH_VSTAGES) * CH_KV_BYTES + (13 + CH_RING) * sizeof(uint64_t) + CH_RING * sizeof(ChunkUnit) + 6 * 4 +
            CH_PHASES * sizeof(ChunkStretch);
 }
-static_assert(CH_RING * sizeof(ChunkUnit) >= 30 * 4, "the sums over the rows lie where the pieces come later");
+static_assert(CH_RING * sizeof(ChunkUnit) >= 36 * 4, "the sums over the rows lie where the pieces come later");
 
 // How a launch of these sizes is cut: what of it doesn't depend on the rows' lengths.
 struct ChunkShape {
     int G, tile_tokens, n_qtiles, grid, phases, phase_pairs, part_rows;
     int ctas;  // of a cluster; 0: no clusters
     long long n_items;
-    size_t plan_bytes;
+    int rounds;
+    size_t plan_bytes, deal_bytes;
 };
 // CTAs to a pair (0: stretches) where rows have one tile of queries: as many as the chip has room for at once (two per SM, some lost between
 // clusters of 4 and 8), if a CTA's key tiles are then few and not many more than a stretch would have.  Lengths aren't known here, a full table is
@@ -1082,10 +1127,13 @@ static ChunkShape chunk_shape(int B, int T, int Hq, int Hkv, long long capacity,
         s.phases = 0;
     }
     s.plan_bytes = ((size_t)s.phases * s.grid * sizeof(ChunkPlan) + 255) / 256 * 256;
+    s.rounds = (int)(s.n_items / s.grid + 1);
+    // (rows of one tile of queries are never dealt, but for the one CTA of a grid of one)
+    s.deal_bytes = s.ctas || (s.n_qtiles == 1 && s.grid > 1) ? 0 : ((size_t)s.grid * s.rounds * sizeof(ChunkDeal) + 255) / 256 * 256;
     return s;
 }
 static size_t chunk_workspace(const ChunkShape &s) {
-    return s.phases ? s.plan_bytes + (size_t)s.phases * 2 * s.grid * s.part_rows * (NCKV_D + 2) * 4 : 0;
+    return s.deal_bytes + (s.phases ? s.plan_bytes + (size_t)s.phases * 2 * s.grid * s.part_rows * (NCKV_D + 2) * 4 : 0);
 }
 static int chunk_check_sizes(const char *name, int B, int T, int Hq, int Hkv, int page_tokens, int max_pages) {
     if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || page_tokens <= 0 || max_pages <= 0) {
@@ -1169,10 +1217,13 @@ extern "C" int nckv_prefill_attn_paged(const void *q, const void *k_pool, const 
     p.new_tokens = new_tokens;
     p.v_pool = static_cast<const __nv_bfloat16 *>(v_pool);
     p.out = static_cast<__nv_bfloat16 *>(out);
-    p.plan = static_cast<ChunkPlan *>(workspace);
+    p.deals = static_cast<ChunkDeal *>(workspace);
+    p.rounds = s.rounds;
+    char *const rest = static_cast<char *>(workspace) + s.deal_bytes;
+    p.plan = reinterpret_cast<ChunkPlan *>(rest);
     p.part_o = p.part_ml = nullptr;
     if (s.phases) {
-        p.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + s.plan_bytes);
+        p.part_o = reinterpret_cast<float *>(rest + s.plan_bytes);
         p.part_ml = p.part_o + (size_t)s.phases * 2 * s.grid * s.part_rows * NCKV_D;
     }
     p.status = status;
