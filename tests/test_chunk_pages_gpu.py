@@ -136,6 +136,29 @@ def test_all_ways_of_sharing_the_work(B, T, Hq, Hkv, lens, window, counts):
         assert not got[b, int(args[5][b]):].any()
 
 
+@pytest.mark.parametrize("T,counts", [(3, True), (40, True), (40, False)])
+def test_the_most_rows_of_a_launch(T, counts):
+    """4096 rows that share two pages, of 8 lengths and 7 counts, in one launch; one more is refused."""
+    from nanochat_b200 import ops
+    B = 4096
+    lens, new = [9 * (i % 8) for i in range(B)], [6 * (i % 7) * T // 40 if counts else T for i in range(B)]
+    q, k, v, table, at, n = make(56, T, 4, 1, 96, lens[:56], seed=T, new=new[:56])
+    pages = torch.randn(2, 96, 1, 128, generator=torch.Generator(device=DEV).manual_seed(T), device=DEV).to(BF)
+    k, v, table = pages, pages.flip(0).contiguous(), torch.tensor([[1, 0]] * B, dtype=torch.int32, device=DEV)
+    kinds = torch.arange(B, device=DEV) % 56
+    args = (q, k, v, table[:56], at, n)
+    want, size = definition(*args, -1)
+    got = ops.prefill_attention_paged(q[kinds], k, v, table, at[kinds].contiguous(), n[kinds].contiguous() if counts else None)
+    assert ops.read_status(DEV) == 0
+    check(got[:56], *args, -1)
+    # every row's error has the room that check() gives
+    err = (got.double() - want[kinds]).abs()
+    assert bool((err <= (2.0 ** -8 * (size + want.abs()) + 2.0 ** -12 * size)[kinds]).all())
+    with pytest.raises(RuntimeError, match="at most 4096"):
+        ops.prefill_attention_paged(q[:1].expand(B + 1, -1, -1, -1), k, v, table[:1].expand(B + 1, -1).contiguous(),
+                                    torch.zeros(B + 1, dtype=torch.int32, device=DEV))
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 def test_values_that_are_not_finite_reach_only_who_sees_them(bad):
     from nanochat_b200 import ops
