@@ -17,7 +17,7 @@
 
 namespace nckv {
 
-constexpr int AD_THREADS = 256, AD_ROWS = 8;
+constexpr int AD_THREADS = 256, AD_ROWS = 8, AD_AHEAD = 4;  // AD_AHEAD: groups of outputs whose y is on its way (1: 256 rows, 8192 outputs at rank 64 take 0.7 us more)
 constexpr int AD_BOX = 32, AD_BOX_BYTES = AD_BOX * 128, AD_STAGES = 3;  // of a warp's ring
 
 struct AdapterRows : AdapterParams {
@@ -59,11 +59,15 @@ __device__ __forceinline__ bool adapter_unit(const AdapterRows &p, int unit, int
         __syncthreads();
         return true;
     }
-    for (int i = tid; i <= p.S; i += AD_THREADS) s_count[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < p.B; i += AD_THREADS) {
+    auto slot_of = [&](int i) {
         const int s = p.slots[i];
-        atomicAdd(&s_count[s < 0 || s >= p.S ? p.S : s], 1);
+        return s < 0 || s >= p.S ? p.S : s;
+    };
+    int mine0 = -1;  // the slot of request tid
+    for (int i = tid; i < p.B; i += AD_THREADS) {  // (the counts are zero)
+        const int s = slot_of(i);
+        if (i == tid) mine0 = s;
+        atomicAdd(&s_count[s], 1);
     }
     __syncthreads();
     // units before each thread's run of slots
@@ -103,8 +107,7 @@ __device__ __forceinline__ bool adapter_unit(const AdapterRows &p, int unit, int
     int found = 0;
     for (int i0 = 0; i0 < p.B && found < first + p.per_unit; i0 += AD_THREADS) {
         const int i = i0 + tid;
-        const int s = i < p.B ? p.slots[i] : -2;
-        const bool member = i < p.B && (s < 0 || s >= p.S ? p.S : s) == which;
+        const bool member = i < p.B && (i0 ? slot_of(i) : mine0) == which;
         const unsigned votes = __ballot_sync(0xffffffffu, member);
         __syncthreads();
         if (lane == 0) s_warp[warp] = __popc(votes);
@@ -148,6 +151,9 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_down, const __grid_c
         fence_mbar_init();
     }
     __syncwarp();
+    if (p.per_unit > 1 && p.B > 32)
+        for (int i = threadIdx.x; i <= p.S; i += AD_THREADS) s_count[i] = 0;
+    __syncthreads();
     pdl_wait_prior_grids();
     pdl_launch_dependents();  // behind the wait: what a next grid reads ahead of its own is older than this one's operands
     const int ctas = (int)cluster_ctas(), rank = (int)cluster_rank();
@@ -238,10 +244,10 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_down, const __grid_c
             next(box);
         }
     }
-    // y of a group of outputs, of the two tokens whose results this lane holds
+    // y of AD_AHEAD groups of outputs, of the two tokens whose results this lane holds
     const int t0 = s_row[quad * 2], t1 = s_row[quad * 2 + 1];
-    uint32_t y[2][2];
-    auto load_y = [&](int step) {
+    uint32_t y_ring[AD_AHEAD][2][2];
+    auto load_y = [&](uint32_t (&y)[2][2], int step) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int n = n_lo + (step * WARPS + warp) * AD_BOX + j * 16 + line * 2;
@@ -250,7 +256,9 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_down, const __grid_c
             if (n < n_hi && t1 >= 0) y[j][1] = *reinterpret_cast<const uint32_t *>(p.y + t1 * p.y_stride + n);
         }
     };
-    if (n_steps > 0) load_y(0);
+#pragma unroll
+    for (int i = 0; i < AD_AHEAD; ++i)
+        if (i < n_steps) load_y(y_ring[i], i);
     // ---- the warps' sums, then the CTAs', in a fixed order ---------------------------------------------
     for (int w0 = 0; w0 < WARPS; w0 += AT_ONCE) {
         if (w0) __syncthreads();
@@ -307,46 +315,51 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_down, const __grid_c
             if (both && line >= 4) hi[i][e] = lo[i][e];
         }
     const float scale = p.scales[slot];
-    for (int step = 0; step < n_steps && ok; ++step) {
-        float o[2][4];
+    for (int step0 = 0; step0 < n_steps && ok; step0 += AD_AHEAD)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+        for (int ahead = 0; ahead < AD_AHEAD; ++ahead) {
+            const int step = step0 + ahead;
+            if (step >= n_steps) break;
+            uint32_t(&y)[2][2] = y_ring[ahead];
+            float o[2][4];
 #pragma unroll
-        for (int part = 0; part < UP_BOXES; ++part, ++box) {
-            const uint32_t at = landed(box);
+            for (int j = 0; j < 2; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int row = j * 16 + m_row * 2 + m_low;
+            for (int part = 0; part < UP_BOXES; ++part, ++box) {
+                const uint32_t at = landed(box);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (part * 4 + i >= STEPS) break;
-                    uint32_t w0, w1, w2, w3;
-                    ldmatrix_x4(w0, w1, w2, w3, at + row * 128 + (((i * 2 + m_half) ^ (row & 7)) << 4));
-                    mma_bf16_16816(o[j][0], o[j][1], o[j][2], o[j][3], w0, w1, w2, w3, hi[part * 4 + i][0], hi[part * 4 + i][1]);
-                    if (!both) mma_bf16_16816(o[j][0], o[j][1], o[j][2], o[j][3], w0, w1, w2, w3, lo[part * 4 + i][0], lo[part * 4 + i][1]);
+                for (int j = 0; j < 2; ++j) {
+                    const int row = j * 16 + m_row * 2 + m_low;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (part * 4 + i >= STEPS) break;
+                        uint32_t w0, w1, w2, w3;
+                        ldmatrix_x4(w0, w1, w2, w3, at + row * 128 + (((i * 2 + m_half) ^ (row & 7)) << 4));
+                        mma_bf16_16816(o[j][0], o[j][1], o[j][2], o[j][3], w0, w1, w2, w3, hi[part * 4 + i][0], hi[part * 4 + i][1]);
+                        if (!both) mma_bf16_16816(o[j][0], o[j][1], o[j][2], o[j][3], w0, w1, w2, w3, lo[part * 4 + i][0], lo[part * 4 + i][1]);
+                    }
                 }
+                next(box);
             }
-            next(box);
-        }
-        if (!ok) break;
-        if (both)
+            if (!ok) break;
+            if (both)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[j][e] += __shfl_xor_sync(0xffffffffu, o[j][e], 2);  // quads 0 and 1: the tokens' first terms
+            uint32_t out[2][2];
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[j][e] += __shfl_xor_sync(0xffffffffu, o[j][e], 2);  // quads 0 and 1: the tokens' first terms
-        uint32_t out[2][2];
+                for (int e = 0; e < 2; ++e) out[j][e] = pack_bf16x2(bf16lo(y[j][e]) + scale * o[j][e], bf16hi(y[j][e]) + scale * o[j][2 + e]);
+            if (step + AD_AHEAD < n_steps) load_y(y, step + AD_AHEAD);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) out[j][e] = pack_bf16x2(bf16lo(y[j][e]) + scale * o[j][e], bf16hi(y[j][e]) + scale * o[j][2 + e]);
-        if (step + 1 < n_steps) load_y(step + 1);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int n = n_lo + (step * WARPS + warp) * AD_BOX + j * 16 + line * 2;
-            if (n < n_hi && t0 >= 0) *reinterpret_cast<uint32_t *>(p.out + t0 * p.out_stride + n) = out[j][0];
-            if (n < n_hi && t1 >= 0) *reinterpret_cast<uint32_t *>(p.out + t1 * p.out_stride + n) = out[j][1];
+            for (int j = 0; j < 2; ++j) {
+                const int n = n_lo + (step * WARPS + warp) * AD_BOX + j * 16 + line * 2;
+                if (n < n_hi && t0 >= 0) *reinterpret_cast<uint32_t *>(p.out + t0 * p.out_stride + n) = out[j][0];
+                if (n < n_hi && t1 >= 0) *reinterpret_cast<uint32_t *>(p.out + t1 * p.out_stride + n) = out[j][1];
+            }
         }
-    }
     if (!ok && lane == 0) {  // a copy did not land in time: the ones behind it may still be under way
         atomicOr(p.status, (int)NCKV_ST_TIMEOUT);
         for (int i = max(fetched - AD_STAGES, 0); i < fetched; ++i) mbar_wait_bounded(&bar[i % AD_STAGES], (i / AD_STAGES) & 1);
