@@ -352,7 +352,7 @@ NCKV_API int nckv_paged_fill(const void *src_k, const void *src_v, void *k_pool,
  * Attention of a chunk of T new tokens per row over pages that hold them already (nckv_append_rope_norm_paged_counts ahead of it).  Row b has
  * cache_seqlens[b] keys before the chunk and new_tokens[b] tokens in it (new_tokens NULL: T); query t < new_tokens[b] of q (B, T, Hq, D) sees the
  * keys of positions [max(0, p - window_left), p], p = cache_seqlens[b] + t (window_left < 0: from 0).  out (B, T, Hq, D) is zero in slots without
- * a token and in rows that don't fit their table (flagged).  Hq / Hkv at most 128.  The workspace (256-byte aligned, at least
+ * a token and in rows that don't fit their table (flagged).  At most 4096 rows, Hq / Hkv at most 128.  The workspace (256-byte aligned, at least
  * nckv_prefill_attn_paged_workspace_bytes, which is 0 where none is needed or the sizes are refused) is the call's own.
  */
 NCKV_API size_t nckv_prefill_attn_paged_workspace_bytes(int B, int T, int Hq, int Hkv, int page_tokens, int max_pages, int window_left);

@@ -1,5 +1,6 @@
 // Low-rank adapters beside a shared projection for requests of many tokens (adapters.cu: few): both launches on the tensor cores
 // (tcgen05, accumulators in tensor memory), bound by the activations' bytes: x read once, y read and written once.
+// 6 x 1531 tokens, 6144 -> 1536 at rank 32 (173 MB): 40 us = 4.3 TB/s; 8 x 2048, 2048 -> 8192 at rank 64 (607 MB): 118 us = 5.1.
 //
 // A tile is 128 tokens of one request.  All operands come by TMA with the 128-byte swizzle over maps of three dimensions (channels, tokens,
 // requests), which clip a request's last tile and fill ranks and channels up with zeros.

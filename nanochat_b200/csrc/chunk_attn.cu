@@ -4,7 +4,7 @@
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^((q . k_j) scale log2(e) - m),   j in [max(0, L + t - window), L + t]
 //
 // for query t < n of a row with L keys before its n new ones.  Running maximum and sum in fp32, one pass over the keys; P is
-// rounded to bf16 (2^-9 of a term of the sum, the type of V) because the tensor core takes it beside V in that type.
+// rounded to bf16 (2^-8 of a term of the sum at most, the type of V) because the tensor core takes it beside V in that type.
 //
 // A tile is CH_M = 128 query rows of one (row, kv head): the G query heads of the group at 128 / G consecutive tokens, row = token * G +
 // head, so keys and values are read once for the whole group.  It walks over its keys in tiles of 64, cut at multiples of 64.  Pages
@@ -13,15 +13,23 @@
 // The pipeline is that of the dense kernel (prefill_attn.cu): two persistent CTAs per SM, a copying thread, a thread that issues S = Q K^T two
 // tiles ahead and O += P V, and one softmax thread per query row that takes its scores out of tensor memory and puts P back over them.
 //
-// What a CTA works through, found by every role from the rows' lengths alone:
+// What a CTA works through, found from the rows' lengths by all of its threads before the first tile:
 //   stretches: the sequence of all key tiles of all tiles of queries, (row, kv head) by (row, kv head), is cut into equal stretches, one per
 //     CTA; tiles of queries that lie in several leave partial sums.  Balanced to a key tile whatever the lengths.  Where tiles of queries share
 //     keys (more than one per row) and the keys are more than L2 holds, up to CH_PHASES groups of pairs are cut one after the other.
 //   a deal: where tiles of queries are many or alike enough to fill the CTAs' rounds they go to the CTAs uncut, back and forth: of rows of like
-//     lengths longest first as in the dense kernel, of others row by row, empty ones left out.
+//     lengths longest first as in the dense kernel, of others row by row, empty ones left out.  A CTA's threads write its list; the copying thread reads an entry ahead.
 //   clusters: few pairs of short rows, one tile of queries each, are bound by launches and round trips.  A cluster takes a pair, each CTA a part of its
 //     keys, and the parts meet in shared memory: no sums over the rows ahead of the work, no launch behind it.
 // chunk_finish_kernel adds up partial sums in the order of the keys: results don't depend on timing.
+//
+// Bounds and figures.  Many new tokens: the tensor pipe and the softmax chain.  A key tile takes the pipe 640 cycles (S 8 products of 48 with both operands
+// in shared memory, O 4 of 64) and the exponentials 512; two CTAs of an SM get through one each in 1680, with the clock at 1.54 GHz under the power limit.
+// 2011 tokens behind 62 000 keys, 16 + 4 heads: 1094 us = 956 TFLOP/s; 8 prompts of 2048, 12 heads: 124 us = 829.  Few new tokens: the keys' bytes.
+// 2 x 8 tokens behind 49 000 keys, 12 heads: 88 us = 6.9 TB/s; 48 x 5 tokens behind 2048, 16 + 4 heads: 49 us = 4.2 TB/s, of which about 14 us are launches,
+// lengths, the first tiles' latency and the sums of parts, whatever the keys.  4 x 4 tokens of short rows: 7.5 us, launch and round trips.
+// Tried and slower: two threads per query row (147 us for the prompts), a warp of its own that cleans edge tiles (155), half or a quarter of the exponentials
+// as polynomials on the FMA pipe (131, 127), a maximum taken from the tile before, scores asked for before the stores of P are waited for (126).
 //
 // Every barrier wait is bounded; one that runs out sets NCKV_ST_TIMEOUT, the CTA stops issuing work, waits for its copies, frees its
 // tensor memory and returns.

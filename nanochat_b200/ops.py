@@ -743,7 +743,7 @@ def decode_attention_paged(q, k_pool, v_pool, block_table, cache_seqlens, seqlen
 def prefill_attention_paged(q, k_pool, v_pool, block_table, cache_seqlens, new_tokens=None, window_left=-1):
     """``prefill_attention`` over paged storage that holds the new keys already: q (B, T, Hq, D), row b's queries at
     positions ``cache_seqlens[b] + t``.  With ``new_tokens`` (int32 per row) only the first ``new_tokens[b]`` of a row's T
-    slots hold a token; the output is zero in the others."""
+    slots hold a token; the output is zero in the others.  At most 4096 rows, 128 query heads to a key/value head."""
     done = _lib.native.prefill_attention_paged(q, k_pool, v_pool, block_table, cache_seqlens, new_tokens, window_left)
     if done is not None:
         return done
@@ -1010,7 +1010,8 @@ def add_adapters(y, x, down, up, slots, scales):
 
 
 def add_adapters_(y, x, down, up, slots, scales):
-    """The same into y, which may be a column slice of a wider product; rows without an adapter are not touched.  Returns y."""
+    """The same into y, which may be a column slice of a wider product and shares no memory with x; rows without an adapter are not
+    touched.  Returns y."""
     if _lib.native.add_adapters(y, x, down, up, slots, scales, True) is not None:
         return y
     _adapters("add_adapters_", y, x, down, up, slots, scales, None)
