@@ -11,7 +11,7 @@
 // its way: boxes of 64 channels of 32 ranks, then 32 outputs by up to 64 ranks.  (By 16-byte asynchronous copies, whose addresses the lanes
 // work out, 256 requests at rank 64 took 32 us where this form of copies took 21; straight from global memory to registers 34.)
 // 256 rows over 48 adapters of rank 64, 2048 -> 8192 (72 MB): 18.9 us = 3.8 TB/s, 2.2 of them until a CTA knows its rows, 4.6 for its part of t, 2 until the
-// parts have met and 7.4 for its part of the outputs; 64 rows of as many adapters, 2048 -> 2048 at rank 16: 7.6; 4 rows of 768 channels: 4.5 (latency).
+// parts have met and 7.4 for its part of the outputs; 64 rows of as many adapters, 2048 -> 2048 at rank 16: 6.7; 4 rows of 768 channels: 4.5 (latency).
 // mma.sync with the weights as the 16 rows and the tokens as the 8 columns (tensor memory would want 128 rows): with the tokens as rows the
 // instruction's rate was the limit.  Up to four tokens have both terms of t in one product.
 #include "adapters.cuh"
@@ -20,6 +20,7 @@
 namespace nckv {
 
 constexpr int AD_THREADS = 256, AD_ROWS = 8, AD_AHEAD = 4;  // AD_AHEAD: groups of outputs whose y is on its way (1: 256 rows, 8192 outputs at rank 64 take 0.7 us more)
+constexpr int AD_TABLE = 256;  // slots up to which requests are counted warp by warp: 2 KB
 constexpr int AD_BOX = 32, AD_BOX_BYTES = AD_BOX * 128, AD_STAGES = 3;  // of a warp's ring
 
 struct AdapterRows : AdapterParams {
@@ -28,13 +29,23 @@ struct AdapterRows : AdapterParams {
     int k_each, n_each;  // channels and outputs of a CTA
 };
 
+// How a unit's rows are found: its number says so; requests compared within a warp; counted warp by warp; counted.  One kernel each: with all of them in
+// one, code that isn't run cost 0.3 of 9 us.
+enum AdapterFind { AD_OWN, AD_WARP, AD_CTA, AD_ANY };
+static AdapterFind adapter_find(int per_unit, int B, int S) {
+    return per_unit == 1 ? AD_OWN : B <= 32 ? AD_WARP : B <= AD_THREADS && S < AD_TABLE ? AD_CTA : AD_ANY;
+}
+// Words of shared memory that requests are counted in.
+__host__ __device__ constexpr int adapter_counts(AdapterFind find, int S) { return find == AD_CTA ? 2 * (S + 1) : find == AD_ANY ? S + 1 : 0; }
+
 // Rows of a unit: row numbers in s_row (-1: none), and its slot (-1: no adapter).  False: there is no such unit.
+template <AdapterFind FIND>
 __device__ __forceinline__ bool adapter_unit(const AdapterRows &p, int unit, int *s_row, int *s_count, int &slot, int &rows) {
     // s_count: requests of each slot, then of none
     __shared__ int s_warp[AD_THREADS / 32], s_which[2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid < AD_ROWS) s_row[tid] = -1;
-    if (p.per_unit == 1) {
+    if constexpr (FIND == AD_OWN) {
         const int b = unit / p.chunks, chunk = unit - b * p.chunks;
         slot = p.slots[b];
         if (slot >= p.S) slot = -1;
@@ -44,7 +55,7 @@ __device__ __forceinline__ bool adapter_unit(const AdapterRows &p, int unit, int
         __syncthreads();
         return true;
     }
-    if (p.B <= 32) {  // every warp: a lane to a request; the first of every per_unit ones of a slot stands for the unit
+    if constexpr (FIND == AD_WARP) {  // every warp: a lane to a request; the first of every per_unit ones of a slot stands for the unit
         const int s0 = lane < p.B ? p.slots[lane] : -2, s = lane >= p.B ? -2 : s0 < 0 || s0 >= p.S ? -1 : s0;
         const unsigned same = __match_any_sync(0xffffffffu, s), below = (1u << lane) - 1;
         const int rank = __popc(same & below);
@@ -65,65 +76,105 @@ __device__ __forceinline__ bool adapter_unit(const AdapterRows &p, int unit, int
         const int s = p.slots[i];
         return s < 0 || s >= p.S ? p.S : s;
     };
-    int mine0 = -1;  // the slot of request tid
-    for (int i = tid; i < p.B; i += AD_THREADS) {  // (the counts are zero)
-        const int s = slot_of(i);
-        if (i == tid) mine0 = s;
-        atomicAdd(&s_count[s], 1);
-    }
-    __syncthreads();
-    // units before each thread's run of slots
-    const int run = (p.S + AD_THREADS) / AD_THREADS, lo = min(tid * run, p.S + 1), hi = min(lo + run, p.S + 1);
-    int mine = 0;
-    for (int i = lo; i < hi; ++i) mine += (s_count[i] + p.per_unit - 1) / p.per_unit;
-    int before = mine;
+    if constexpr (FIND == AD_CTA) {  // a thread to a request, then to a slot
+        unsigned long long *s_table = reinterpret_cast<unsigned long long *>(s_count);  // (zero) requests of each slot, a byte to a warp
+        auto sum = [](unsigned long long c) { return (int)__dp4a((unsigned)c, 0x01010101u, __dp4a((unsigned)(c >> 32), 0x01010101u, 0u)); };
+        const int s = tid < p.B ? slot_of(tid) : -1;
+        const unsigned same = __match_any_sync(0xffffffffu, s), below = same & ((1u << lane) - 1);
+        if (s >= 0 && !below) reinterpret_cast<uint8_t *>(s_table + s)[warp] = (uint8_t)__popc(same);
+        __syncthreads();
+        // requests of the slot ahead of this one; units of this thread's slot
+        const int rank = __popc(below) + (s >= 0 ? sum(s_table[s] & ((1ull << (8 * warp)) - 1)) : 0);
+        const int units = tid <= p.S ? (sum(s_table[tid]) + p.per_unit - 1) / p.per_unit : 0;
+        int before = units;
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, before, off);
-        if (lane >= off) before += v;
-    }
-    if (lane == 31) s_warp[warp] = before;
-    __syncthreads();
-    int all = 0;
-    before -= mine;
-    for (int w = 0; w < AD_THREADS / 32; ++w) {
-        if (w < warp) before += s_warp[w];
-        all += s_warp[w];
-    }
-    if (unit >= all) return false;
-    if (unit >= before && unit < before + mine) {
-        int i = lo;
-        for (;; ++i) {
-            const int n = (s_count[i] + p.per_unit - 1) / p.per_unit;
-            if (unit < before + n) break;
-            before += n;
+        for (int off = 1; off < 32; off <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, before, off);
+            if (lane >= off) before += v;
         }
-        s_which[0] = i;
-        s_which[1] = unit - before;
-    }
-    __syncthreads();
-    const int which = s_which[0], first = s_which[1] * p.per_unit;
-    slot = which < p.S ? which : -1;
-    rows = min(s_count[which] - first, p.per_unit) * p.T;
-    // its members: the requests of the slot from the first-th on, in order
-    int found = 0;
-    for (int i0 = 0; i0 < p.B && found < first + p.per_unit; i0 += AD_THREADS) {
-        const int i = i0 + tid;
-        const bool member = i < p.B && (i0 ? slot_of(i) : mine0) == which;
-        const unsigned votes = __ballot_sync(0xffffffffu, member);
+        if (lane == 31) s_warp[warp] = before;
         __syncthreads();
-        if (lane == 0) s_warp[warp] = __popc(votes);
-        __syncthreads();
-        int at = found - first + __popc(votes & ((1u << lane) - 1));
+        before -= units;
+        int all = 0;
         for (int w = 0; w < AD_THREADS / 32; ++w) {
-            if (w < warp) at += s_warp[w];
-            found += s_warp[w];
+            if (w < warp) before += s_warp[w];
+            all += s_warp[w];
         }
-        if (member && at >= 0 && at < p.per_unit)
-            for (int t = 0; t < p.T; ++t) s_row[at * p.T + t] = i * p.T + t;
+        if (unit >= all) return false;
+        if (unit >= before && unit < before + units) {
+            s_which[0] = tid;
+            s_which[1] = (unit - before) * p.per_unit;
+        }
+        __syncthreads();
+        const int which = s_which[0], first = s_which[1];
+        slot = which < p.S ? which : -1;
+        const bool member = s == which && rank >= first && rank < first + p.per_unit;
+        if (member)
+            for (int t = 0; t < p.T; ++t) s_row[(rank - first) * p.T + t] = tid * p.T + t;
+        rows = __syncthreads_count(member) * p.T;
+        return true;
     }
-    __syncthreads();
-    return true;
+    if constexpr (FIND == AD_ANY) {
+        int mine0 = -1;  // the slot of request tid
+        for (int i = tid; i < p.B; i += AD_THREADS) {  // (the counts are zero)
+            const int s = slot_of(i);
+            if (i == tid) mine0 = s;
+            atomicAdd(&s_count[s], 1);
+        }
+        __syncthreads();
+        // units before each thread's run of slots
+        const int run = (p.S + AD_THREADS) / AD_THREADS, lo = min(tid * run, p.S + 1), hi = min(lo + run, p.S + 1);
+        int mine = 0;
+        for (int i = lo; i < hi; ++i) mine += (s_count[i] + p.per_unit - 1) / p.per_unit;
+        int before = mine;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, before, off);
+            if (lane >= off) before += v;
+        }
+        if (lane == 31) s_warp[warp] = before;
+        __syncthreads();
+        int all = 0;
+        before -= mine;
+        for (int w = 0; w < AD_THREADS / 32; ++w) {
+            if (w < warp) before += s_warp[w];
+            all += s_warp[w];
+        }
+        if (unit >= all) return false;
+        if (unit >= before && unit < before + mine) {
+            int i = lo;
+            for (;; ++i) {
+                const int n = (s_count[i] + p.per_unit - 1) / p.per_unit;
+                if (unit < before + n) break;
+                before += n;
+            }
+            s_which[0] = i;
+            s_which[1] = unit - before;
+        }
+        __syncthreads();
+        const int which = s_which[0], first = s_which[1] * p.per_unit;
+        slot = which < p.S ? which : -1;
+        rows = min(s_count[which] - first, p.per_unit) * p.T;
+        // its members: the requests of the slot from the first-th on, in order
+        int found = 0;
+        for (int i0 = 0; i0 < p.B && found < first + p.per_unit; i0 += AD_THREADS) {
+            const int i = i0 + tid;
+            const bool member = i < p.B && (i0 ? slot_of(i) : mine0) == which;
+            const unsigned votes = __ballot_sync(0xffffffffu, member);
+            __syncthreads();
+            if (lane == 0) s_warp[warp] = __popc(votes);
+            __syncthreads();
+            int at = found - first + __popc(votes & ((1u << lane) - 1));
+            for (int w = 0; w < AD_THREADS / 32; ++w) {
+                if (w < warp) at += s_warp[w];
+                found += s_warp[w];
+            }
+            if (member && at >= 0 && at < p.per_unit)
+                for (int t = 0; t < p.T; ++t) s_row[at * p.T + t] = i * p.T + t;
+        }
+        __syncthreads();
+        return true;
+    }
 }
 
 // What the second term of t holds; nothing beside an infinity, whose rest would be NaN.
@@ -131,7 +182,7 @@ __device__ __forceinline__ float adapter_rest(float t, float hi) { return fabsf(
 
 // Down: a warp takes every eighth step of 64 channels.  Up: a warp takes every eighth group of 32 outputs; row i of product j is output
 // j * 16 + i % 8 * 2 + i / 8 of the 32, so that a lane holds 2 consecutive ones of a token.
-template <int STEPS>  // of 16 ranks
+template <int STEPS, AdapterFind FIND>  // steps of 16 ranks
 __global__ void __launch_bounds__(AD_THREADS, 2)
 adapter_rows_kernel(const __grid_constant__ CUtensorMap map_down, const __grid_constant__ CUtensorMap map_up, const __grid_constant__ AdapterRows p) {
     constexpr int RANKS = 16 * STEPS, PITCH = RANKS + 4, WARPS = AD_THREADS / 32;
@@ -153,14 +204,13 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_down, const __grid_c
         fence_mbar_init();
     }
     __syncwarp();
-    if (p.per_unit > 1 && p.B > 32)
-        for (int i = threadIdx.x; i <= p.S; i += AD_THREADS) s_count[i] = 0;
+    for (int i = threadIdx.x; i < adapter_counts(FIND, p.S); i += AD_THREADS) s_count[i] = 0;
     __syncthreads();
     pdl_wait_prior_grids();
     pdl_launch_dependents();  // behind the wait: what a next grid reads ahead of its own is older than this one's operands
     const int ctas = (int)cluster_ctas(), rank = (int)cluster_rank();
     int slot, rows;
-    if (!adapter_unit(p, blockIdx.x / ctas, s_row, s_count, slot, rows)) return;  // all of the cluster's CTAs
+    if (!adapter_unit<FIND>(p, blockIdx.x / ctas, s_row, s_count, slot, rows)) return;  // all of the cluster's CTAs
     const int n_lo = rank * p.n_each, n_hi = min(n_lo + p.n_each, p.N);
     if (slot < 0 || (smem_u32(smem) & 1023u) != 0) {
         if (slot >= 0 && threadIdx.x == 0) atomicOr(p.status, (int)NCKV_ST_TIMEOUT);  // checked rather than assumed
@@ -370,6 +420,13 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_down, const __grid_c
     if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the others have read this one's
 }
 
+using AdapterKernel = void (*)(CUtensorMap, CUtensorMap, AdapterRows);
+template <int STEPS>
+static AdapterKernel adapter_kernel(AdapterFind find) {
+    return find == AD_OWN ? adapter_rows_kernel<STEPS, AD_OWN> : find == AD_WARP ? adapter_rows_kernel<STEPS, AD_WARP>
+         : find == AD_CTA ? adapter_rows_kernel<STEPS, AD_CTA> : adapter_rows_kernel<STEPS, AD_ANY>;
+}
+
 // Units at most: the requests are known here, their slots aren't.
 static long long adapter_units(int B, int T, int S, int *per_unit, int *chunks) {
     *chunks = (T + AD_ROWS - 1) / AD_ROWS;
@@ -459,16 +516,17 @@ extern "C" int nckv_adapters(const void *y, int64_t y_stride, const void *x, int
     rc = make_tensor_map(&map_down, down, 3, down_dims, down_strides, box);
     if (rc == NCKV_OK) rc = make_tensor_map(&map_up, up, 3, up_dims, up_strides, box);
     if (rc != NCKV_OK) return rc;
+    const AdapterFind find = adapter_find(p.per_unit, B, S);
     const int steps = R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8, at_once = steps <= 2 ? 8 : 16 / steps, warps = AD_THREADS / 32;
     const size_t smem = (size_t)warps * AD_STAGES * AD_BOX_BYTES + (size_t)(1 + at_once) * AD_ROWS * (16 * steps + 4) * 4 + warps * AD_STAGES * 8 +
-                        (p.per_unit > 1 && B > 32 ? (size_t)(S + 1) * 4 : 0);
-    const auto kernel = steps == 1 ? adapter_rows_kernel<1> : steps == 2 ? adapter_rows_kernel<2> : steps == 4 ? adapter_rows_kernel<4> : adapter_rows_kernel<8>;
-    static bool attr_set[64][9] = {};
+                        (size_t)adapter_counts(find, S) * 4;
+    const auto kernel = steps == 1 ? adapter_kernel<1>(find) : steps == 2 ? adapter_kernel<2>(find) : steps == 4 ? adapter_kernel<4>(find) : adapter_kernel<8>(find);
+    static bool attr_set[64][9][4] = {};
     int dev = 0;
     NCKV_CUDA_CHECK(cudaGetDevice(&dev));
-    if (dev >= 64 || !attr_set[dev][steps]) {
+    if (dev >= 64 || !attr_set[dev][steps][find]) {
         NCKV_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-        if (dev < 64) attr_set[dev][steps] = true;
+        if (dev < 64) attr_set[dev][steps][find] = true;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(units * ctas));

@@ -92,6 +92,20 @@ def test_many_requests_of_one_adapter():
         check(ops.add_adapters(*args), *args)
 
 
+@pytest.mark.parametrize("B", [33, 250, 256, 257, 600])
+@pytest.mark.parametrize("S", [2, 255, 256, 300])
+@pytest.mark.parametrize("T", [1, 3])
+def test_all_ways_of_counting_requests(B, S, T):
+    """Many requests of few slots beside slots of one request, in any order."""
+    from nanochat_b200 import ops
+    gen = torch.Generator().manual_seed(B + S)
+    slots = torch.where(torch.rand(B, generator=gen) < 0.5, torch.randint(-1, 2, (B,), generator=gen), torch.randint(-1, S, (B,), generator=gen)).tolist()
+    args = make(B, T, 72, 136, 8, S, seed=B + S, slots=slots)
+    got = ops.add_adapters(*args)
+    assert ops.read_status(DEV) == 0
+    check(got, *args)
+
+
 def test_a_row_does_not_depend_on_its_batch():
     from nanochat_b200 import ops
     y, x, down, up, slots, scales = make(20, 1, 512, 768, 16, 3, seed=1, slots=[i % 3 for i in range(20)])
