@@ -10,7 +10,7 @@
 // part of the weights through a ring of its own by TMA, `up` right behind `down`, so that the first outputs' weights arrive while t is still on
 // its way: boxes of 64 channels of 32 ranks, then 32 outputs by up to 64 ranks.  (By 16-byte asynchronous copies, whose addresses the lanes
 // work out, 256 requests at rank 64 took 32 us where this form of copies took 21; straight from global memory to registers 34.)
-// 256 rows over 48 adapters of rank 64, 2048 -> 8192 (72 MB): 18.9 us = 3.8 TB/s, 2.2 of them until a CTA knows its rows, 4.6 for its part of t, 2 until the
+// 256 rows over 48 adapters of rank 64, 2048 -> 8192 (72 MB): 19.1 us = 3.8 TB/s, 1.5 of them until a CTA knows its rows, 4.6 for its part of t, 2 until the
 // parts have met and 7.4 for its part of the outputs; 64 rows of as many adapters, 2048 -> 2048 at rank 16: 6.7; 4 rows of 768 channels: 4.5 (latency).
 // mma.sync with the weights as the 16 rows and the tokens as the 8 columns (tensor memory would want 128 rows): with the tokens as rows the
 // instruction's rate was the limit.  Up to four tokens have both terms of t in one product.
@@ -19,7 +19,7 @@
 
 namespace nckv {
 
-constexpr int AD_THREADS = 256, AD_ROWS = 8, AD_AHEAD = 4;  // AD_AHEAD: groups of outputs whose y is on its way (1: 256 rows, 8192 outputs at rank 64 take 0.7 us more)
+constexpr int AD_THREADS = 256, AD_ROWS = 8, AD_AHEAD = 4;  // AD_AHEAD: groups of outputs whose y is on its way (1: 256 rows, 8192 outputs at rank 64 take 0.4 us more)
 constexpr int AD_TABLE = 256;  // slots up to which requests are counted warp by warp: 2 KB
 constexpr int AD_BOX = 32, AD_BOX_BYTES = AD_BOX * 128, AD_STAGES = 3;  // of a warp's ring
 
