@@ -18,7 +18,7 @@
 //     CTA; tiles of queries that lie in several leave partial sums.  Balanced to a key tile whatever the lengths.  Where tiles of queries share
 //     keys (more than one per row) and the keys are more than L2 holds, up to CH_PHASES groups of pairs are cut one after the other.
 //   a deal: where tiles of queries are many or alike enough to fill the CTAs' rounds they go to the CTAs uncut, back and forth: of rows of like
-//     lengths longest first as in the dense kernel, of others row by row, empty ones left out.  A CTA's threads write its list; the copying thread reads an entry ahead.
+//     lengths longest first as in the dense kernel, of others row by row, empty ones left out, a last round of few long tiles cut into stretches.  A CTA's threads write its list; the copying thread reads an entry ahead.
 //   clusters: few pairs of short rows, one tile of queries each, are bound by launches and round trips.  A cluster takes a pair, each CTA a part of its
 //     keys, and the parts meet in shared memory: no sums over the rows ahead of the work, no launch behind it.
 // chunk_finish_kernel adds up partial sums in the order of the keys: results don't depend on timing.
@@ -61,8 +61,9 @@ struct alignas(16) ChunkPlan {  // a CTA's stretch of a phase: its first key til
     int n, none[3];                               // new tokens of the row
 };
 
-struct alignas(16) ChunkDeal {  // an uncut tile of queries: row (-1: nothing), kv head + Hkv * number of the tile, the row's lengths
+struct alignas(16) ChunkDeal {  // a tile of queries: row (-1: nothing), kv head + Hkv * number of the tile, the row's lengths; the part of its key tiles
     int b, local, L, n;
+    int off, n_tiles, slot, none;  // n_tiles 0: all of them
 };
 
 struct ChunkParams {
@@ -70,8 +71,8 @@ struct ChunkParams {
     const __nv_bfloat16 *v_pool;
     __nv_bfloat16 *out;
     ChunkPlan *plan;    // (phases, CTAs): how the stretches were cut
-    ChunkDeal *deals;   // (CTAs, rounds): what was dealt
-    int rounds;
+    ChunkDeal *deals;   // (CTAs, deal_room): what was dealt
+    int deal_room;
     float *part_ml;  // (slots, part_rows, 2): maximum and sum
     float *part_o;   // (slots, part_rows, 128), not divided by the sum
     int32_t *status;
@@ -169,7 +170,7 @@ struct ChunkCursor {
         phase = deals < 0 ? 0 : -1;
         valid = true;
         if (deals < 0) valid = enter(p, stretches);
-        else if (deals > 0) next_deal = p.deals[(long long)blockIdx.x * p.rounds];
+        else if (deals > 0) next_deal = p.deals[(long long)blockIdx.x * p.deal_room];
         if (valid) load(p, stretches);
     }
     __device__ __forceinline__ void load(const ChunkParams &p, const ChunkStretch *stretches) {
@@ -209,7 +210,7 @@ struct ChunkCursor {
                 return;
             }
             const ChunkDeal d = next_deal;
-            if (++at < end) next_deal = p.deals[(long long)blockIdx.x * p.rounds + at];
+            if (++at < end) next_deal = p.deals[(long long)blockIdx.x * p.deal_room + at];
             if (d.b < 0) continue;
             u.b = d.b;
             u.L = d.L;
@@ -219,9 +220,9 @@ struct ChunkCursor {
             item(p);
             u.kv_lo = span.kv_lo;
             u.kv_hi = span.kv_hi;
-            u.n_tiles = span.count;
-            u.tile0 = span.first;
-            u.slot = -1;
+            u.n_tiles = d.n_tiles ? d.n_tiles : span.count;
+            u.tile0 = span.first + d.off;
+            u.slot = d.slot;
             return;
         }
     }
@@ -231,13 +232,17 @@ struct ChunkCursor {
     __device__ __forceinline__ bool last_of_unit() const { return t == u.n_tiles - 1; }
 };
 
-// Whether uncut tiles dealt to the CTAs take less than stretches (0): 1 in the order of like rows, 2 row by row.  Rows' key tiles per kv head lie
+// Whether uncut tiles dealt to the CTAs take less than stretches (0): 1 in the order of like rows, 2 row by row, 3 row by row with the last round, if it
+// is short, cut into stretches of at least CH_REST key tiles (3: 61 us where 6 and 12 take 57, window 512).  Rows' key tiles per kv head lie
 // between `least` and `most`; `items` tiles of queries have `tiles` key tiles altogether.  A piece costs some 2 tiles, a phase of stretches
 // CH_CUT for the partial sums that it leaves (twice 64 KB per CTA, written and read) and the launch that adds them up.  us as stretches / like
 // rows / row by row, window -1: 8 x 2048 tokens, 12 + 12 heads, no context 215 / 126 / 170; 2 x 1722, 10 + 1 heads 52 / 37 / 40; 8 x 862, 10 + 1, contexts of
 // 0 to 114 67 / 38 / 47; 2011 behind 60000, 16 + 4 1088 / 1139 / 1147; up to 1931 new tokens in 5 rows, 6 + 6 50 / 45 / 39; 24 x up to 384, 16 + 4, window 1024
-// 113 / 103 / 85; 21 x up to 220 behind up to 3019, 12 + 12 91 / 100 / 99.
+// 113 / 103 / 85; 21 x up to 220 behind up to 3019, 12 + 12 91 / 100 / 99.  A last round of few tiles runs faster than the others, so it is cut only where it
+// saves CH_REST_CUT: 24 x up to 384 behind up to 8192, 16 + 4 heads, row by row / with the last round cut, window 2048 132 / 122, window 1024 82 / 85.
 constexpr float CH_CUT = 25.f;
+constexpr int CH_REST = 6, CH_REST_TILES = 2;  // tiles of queries of a last round to a thread
+constexpr float CH_REST_CUT = 16.f;
 __device__ __forceinline__ int chunk_dealt(const ChunkParams &p, int least, int most, long long tiles, int items, int longest, int grid) {
     if (p.phases == 0) return 1;
     if (p.n_qtiles == 1 || items == 0) return 0;
@@ -245,6 +250,10 @@ __device__ __forceinline__ int chunk_dealt(const ChunkParams &p, int least, int 
     const bool like_rows = !p.new_tokens && most - least <= most / 3;
     const bool alike = longest < 1.5f * each;  // then rounds are whole, else the short tiles fill them up, longest first or not
     const float deal = alike ? ceilf(rounds) * (each + 2.f) : like_rows ? fmaxf(per_cta * 1.05f, (float)longest) + 2.f * rounds : per_cta + longest + 2.f * rounds;
+    if (!like_rows && alike && items > grid && grid <= CH_REST_TILES * CH_THREADS) {
+        const float full = floorf(rounds), rest = full * (each + 2.f) + fmaxf((rounds - full) * each, (float)CH_REST) + CH_REST_CUT;
+        if (rest < fminf(deal, per_cta + 2.f * rounds + CH_CUT * p.phases)) return 3;
+    }
     return deal <= per_cta + 2.f * rounds + CH_CUT * p.phases ? 2 - like_rows : 0;
 }
 
@@ -446,37 +455,88 @@ chunk_attn_kernel(const __grid_constant__ ChunkMaps maps, const __grid_constant_
     __syncthreads();
     if (dealt) {
         // a thread to a round; dealt back and forth
-        const int pairs = p.B * p.Hkv, per_group = p.group_pairs * p.n_qtiles, limit = dealt == 2 ? items : pairs * p.n_qtiles;
-        const int grid = (int)gridDim.x, c = (int)blockIdx.x;
+        const int pairs = p.B * p.Hkv, per_group = p.group_pairs * p.n_qtiles, grid = (int)gridDim.x, c = (int)blockIdx.x;
+        const int limit = dealt == 1 ? pairs * p.n_qtiles : dealt == 2 ? items : items / grid * grid;
+        ChunkDeal *mine = p.deals + (long long)c * p.deal_room;
+        auto row_by_row = [&](int idx) {
+            int lo = 0, hi = p.B - 1;  // the first row with tiles behind idx
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                if (s_items[mid + 1] > idx) hi = mid;
+                else lo = mid + 1;
+            }
+            const ChunkRow r = chunk_row(p, lo);
+            const int in_row = idx - s_items[lo], qt = (r.n + p.tile_tokens - 1) / p.tile_tokens - 1 - in_row / p.Hkv;  // longest first
+            return ChunkDeal{lo, qt * p.Hkv + in_row % p.Hkv, r.L, r.n, 0, 0, -1, 0};
+        };
         deals = limit / grid;
         deals += ((deals & 1) ? grid - 1 - c : c) < limit - deals * grid;
         for (int i = tid; i < deals; i += CH_THREADS) {
             const int idx = i * grid + ((i & 1) ? grid - 1 - c : c);
-            ChunkDeal d;
-            if (dealt == 2) {
-                int lo = 0, hi = p.B - 1;  // the first row with tiles behind idx
-                while (lo < hi) {
-                    const int mid = (lo + hi) / 2;
-                    if (s_items[mid + 1] > idx) hi = mid;
-                    else lo = mid + 1;
-                }
-                d.b = lo;
-                const ChunkRow r = chunk_row(p, lo);
-                const int in_row = idx - s_items[lo], qt = (r.n + p.tile_tokens - 1) / p.tile_tokens - 1 - in_row / p.Hkv;  // longest first
-                d.local = qt * p.Hkv + in_row % p.Hkv;
-                d.L = r.L;
-                d.n = r.n;
-            } else {
+            if (dealt == 1) {
                 const int grp = min(idx / per_group, p.n_groups - 1), in_grp = idx - grp * per_group;
                 const int grp_pairs = grp == p.n_groups - 1 ? pairs - grp * p.group_pairs : p.group_pairs;
                 const int pair = grp * p.group_pairs + in_grp % grp_pairs, qt = p.n_qtiles - 1 - in_grp / grp_pairs;  // all pairs' longest tiles first
                 const ChunkRow r = chunk_row(p, pair / p.Hkv);
-                d.b = qt * p.tile_tokens < r.n ? pair / p.Hkv : -1;
-                d.local = qt * p.Hkv + pair % p.Hkv;
-                d.L = r.L;
-                d.n = r.n;
+                mine[i] = ChunkDeal{qt * p.tile_tokens < r.n ? pair / p.Hkv : -1, qt * p.Hkv + pair % p.Hkv, r.L, r.n, 0, 0, -1, 0};
+            } else mine[i] = row_by_row(idx);
+        }
+        if (dealt == 3) {  // the last round's key tiles one behind the other, CH_REST_TILES of its tiles of queries to a thread
+            ChunkDeal d[CH_REST_TILES];
+            int count[CH_REST_TILES], before = 0, sum = 0;
+#pragma unroll
+            for (int j = 0; j < CH_REST_TILES; ++j) {
+                const int idx = limit + tid * CH_REST_TILES + j;
+                count[j] = 0;
+                if (idx < items) {
+                    d[j] = row_by_row(idx);
+                    count[j] = chunk_span(p, ChunkRow{d[j].L, d[j].n}, d[j].local / p.Hkv * p.tile_tokens).count;
+                }
+                sum += count[j];
             }
-            p.deals[(long long)c * p.rounds + i] = d;
+            before = sum;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, before, off);
+                if (lane >= off) before += v;
+            }
+            if (lane == 31) s_sum[warp] = before;
+            __syncthreads();
+            before -= sum;
+            int total = 0;
+            for (int w = 0; w < CH_THREADS / 32; ++w) {
+                if (w < warp) before += s_sum[w];
+                total += s_sum[w];
+            }
+            const int each = max((total + grid - 1) / grid, CH_REST), from = (int)min((long long)c * each, (long long)total), end = min(from + each, total);
+#pragma unroll
+            for (int j = 0; j < CH_REST_TILES; ++j) {
+                const int upto = before + count[j], number = tid * CH_REST_TILES + j;
+                if (from < end && from >= before && from < upto) {
+                    s_sum[8] = number;
+                    const int hkv = d[j].local % p.Hkv, t0 = d[j].local / p.Hkv * p.tile_tokens;
+                    p.plan[c] = ChunkPlan{from, from - before, count[j], d[j].b, hkv, t0, 0, each, d[j].n, {0, 0, 0}};
+                }
+                if (from < end && end > before && end <= upto) s_sum[9] = number;
+                before = upto;
+            }
+            __syncthreads();
+            if (from < end) {
+                const int first = s_sum[8];
+                before -= sum;
+#pragma unroll
+                for (int j = 0; j < CH_REST_TILES; ++j) {
+                    const int lo = max(from, before), hi = min(end, before + count[j]);
+                    if (lo < hi) {
+                        d[j].off = lo - before;
+                        d[j].n_tiles = hi - lo;
+                        d[j].slot = hi - lo == count[j] ? -1 : c * 2 + (lo != from);
+                        mine[deals + tid * CH_REST_TILES + j - first] = d[j];
+                    }
+                    before += count[j];
+                }
+                deals += s_sum[9] - first + 1;
+            }
         }
     }
     // A warp to a phase: its stretch of this CTA.
@@ -1089,7 +1149,7 @@ struct ChunkShape {
     int G, tile_tokens, n_qtiles, grid, phases, phase_pairs, part_rows;
     int ctas;  // of a cluster; 0: no clusters
     long long n_items;
-    int rounds;
+    int deal_room;
     size_t plan_bytes, deal_bytes;
 };
 // CTAs to a pair (0: stretches) where rows have one tile of queries: as many as the chip has room for at once (two per SM, some lost between
@@ -1135,9 +1195,9 @@ static ChunkShape chunk_shape(int B, int T, int Hq, int Hkv, long long capacity,
         s.phases = 0;
     }
     s.plan_bytes = ((size_t)s.phases * s.grid * sizeof(ChunkPlan) + 255) / 256 * 256;
-    s.rounds = (int)(s.n_items / s.grid + 1);
+    s.deal_room = (int)(s.n_items / s.grid + 1) + s.grid;  // (a last round that is cut: fewer parts than it has tiles)
     // (rows of one tile of queries are never dealt, but for the one CTA of a grid of one)
-    s.deal_bytes = s.ctas || (s.n_qtiles == 1 && s.grid > 1) ? 0 : ((size_t)s.grid * s.rounds * sizeof(ChunkDeal) + 255) / 256 * 256;
+    s.deal_bytes = s.ctas || (s.n_qtiles == 1 && s.grid > 1) ? 0 : ((size_t)s.grid * s.deal_room * sizeof(ChunkDeal) + 255) / 256 * 256;
     return s;
 }
 static size_t chunk_workspace(const ChunkShape &s) {
@@ -1226,7 +1286,7 @@ extern "C" int nckv_prefill_attn_paged(const void *q, const void *k_pool, const 
     p.v_pool = static_cast<const __nv_bfloat16 *>(v_pool);
     p.out = static_cast<__nv_bfloat16 *>(out);
     p.deals = static_cast<ChunkDeal *>(workspace);
-    p.rounds = s.rounds;
+    p.deal_room = s.deal_room;
     char *const rest = static_cast<char *>(workspace) + s.deal_bytes;
     p.plan = reinterpret_cast<ChunkPlan *>(rest);
     p.part_o = p.part_ml = nullptr;

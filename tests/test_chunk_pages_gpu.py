@@ -136,6 +136,31 @@ def test_all_ways_of_sharing_the_work(B, T, Hq, Hkv, lens, window, counts):
         assert not got[b, int(args[5][b]):].any()
 
 
+@pytest.mark.parametrize("B,T,Hq,Hkv,L,window", [
+    (80, 64, 16, 4, 2600, 2500),   # 640 tiles of like length
+    (19, 140, 16, 16, 3000, 1500),  # 608
+    (25, 60, 128, 4, 2300, 2200),  # 1500, four tokens each
+    (300, 70, 8, 1, 2000, 2500),   # 1500
+    (30, 330, 16, 4, 1500, 1400),  # 1320
+])
+def test_a_short_last_round_of_uneven_rows(B, T, Hq, Hkv, L, window):
+    """Tiles of like length that fill the chip's CTAs some times over and a few more, with counts per row; rows share a pool of pages."""
+    from nanochat_b200 import ops
+    kinds = 5
+    lens, new = [L - 64 * i for i in range(kinds)], [T, T, T - 1, T, T - 5]
+    q, k, v, table, at, n = make(kinds, T, Hq, Hkv, 96, lens, seed=T, new=new)
+    which = torch.arange(B, device=DEV) % kinds
+    got = ops.prefill_attention_paged(q[which], k, v, table[which].contiguous(), at[which].contiguous(), n[which].contiguous(), window)
+    assert ops.read_status(DEV) == 0
+    want, size = definition(q, k, v, table, at, n, window)
+    err = (got.double() - want[which]).abs()
+    assert bool((err <= (2.0 ** -8 * (size + want.abs()) + 2.0 ** -12 * size)[which]).all())  # check()'s room
+    for b in range(B):
+        assert not got[b, int(n[b % kinds]):].any()
+    again = ops.prefill_attention_paged(q[which], k, v, table[which].contiguous(), at[which].contiguous(), n[which].contiguous(), window)
+    assert torch.equal(got.view(torch.int16), again.view(torch.int16))
+
+
 @pytest.mark.parametrize("T,counts", [(3, True), (40, True), (40, False)])
 def test_the_most_rows_of_a_launch(T, counts):
     """4096 rows that share two pages, of 8 lengths and 7 counts, in one launch; one more is refused."""
