@@ -355,12 +355,17 @@ class GPT(nn.Module):
         else:
             prev = kv_cache.prev_embedding
             kv_cache.prev_embedding = x[:, -1:, :]
-            if T > 1:
+            if T <= 1:
+                before = prev
+            elif prev is not None and getattr(kv_cache, "paged", False):  # a chunk behind tokens
+                before = torch.cat([prev.expand(B, -1, -1), x[:, :-1]], dim=1)
+            else:  # the start of a sequence, and any chunk into dense rows, as gpt.py:438-449 has it
+                before = None
                 gate = self.smear_lambda.to(x.dtype) * torch.sigmoid(self.smear_gate(x[:, 1:, :24]))
                 x = torch.cat([x[:, :1], x[:, 1:] + gate * x[:, :-1]], dim=1)
-            elif prev is not None:
+            if before is not None:
                 gate = self.smear_lambda.to(x.dtype) * torch.sigmoid(self.smear_gate(x[:, :, :24]))
-                x = x + gate * prev
+                x = x + gate * before
         x0 = x
         backout_at = self.config.n_layer // 2
         x_backout = None
