@@ -41,7 +41,7 @@ def sharded_prefill(prompt_cache, local_cache, group=None, src=0):
     """``KVCache.prefill`` (engine.py:123-137) when the sample rows are spread over ranks.
 
     Rank ``src`` holds the batch-1 cache of the prompt (``prompt_cache``; the others pass None).
-    Its keys and values (and the smear state) are sent ONCE to every rank with a broadcast, land in
+    Its keys and values (and the smear state and the adapter) are sent ONCE to every rank with a broadcast, land in
     that rank's own memory, and each rank then fills its own rows from the local copy with the
     broadcast-copy kernel -- no rank reads another GPU's memory inside a kernel.  ``local_cache``
     is this rank's (empty) KVCache for its share of the rows (``shard_rows``).  Returns the prompt
@@ -50,13 +50,17 @@ def sharded_prefill(prompt_cache, local_cache, group=None, src=0):
     from .engine import KVCache
     rank = dist.get_rank(group)
     dev = local_cache.k_cache.device
-    meta = torch.zeros(2, dtype=torch.int64, device=dev)
+    meta = torch.zeros(4, dtype=torch.int64, device=dev)  # tokens; smear state's width; whether there is an adapter, and its slot
     if rank == src:
         assert prompt_cache is not None and prompt_cache.batch_size == 1, "the source is a batch-1 prompt cache"
         meta[0] = prompt_cache.get_pos()
         meta[1] = 0 if prompt_cache.prev_embedding is None else prompt_cache.prev_embedding.size(-1)
+        slots = getattr(prompt_cache, "adapter_slots", None)
+        if slots is not None:
+            meta[2] = 1
+            meta[3:].copy_(slots)
     dist.broadcast(meta, src=src, group=group)
-    p, emb = int(meta[0]), int(meta[1])
+    p, emb, adapted, slot = meta.tolist()
     if rank == src:
         staged = prompt_cache
     else:
@@ -65,6 +69,8 @@ def sharded_prefill(prompt_cache, local_cache, group=None, src=0):
         staged.cache_seqlens.fill_(p)
         if emb:
             staged.prev_embedding = torch.empty(1, 1, emb, device=dev, dtype=local_cache.k_cache.dtype)
+        if adapted:
+            staged.adapter_slots = torch.tensor([slot], dtype=torch.int32, device=dev)
     if p > 0:
         # only the filled part of the source travels: (L, 1, p, H, D) for K and for V
         k_part = staged.k_cache[:, :, :p].contiguous()
