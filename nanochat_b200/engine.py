@@ -572,7 +572,8 @@ class GraphedDecodeStep:
     ``step(ids)`` copies the token ids into the graph's input buffer, replays, and returns the
     logits buffer (B, vocab) — overwritten by the next call.  The smear state of a KVCache
     (``kv_cache.prev_embedding``) is kept in a persistent buffer that the graph reads and updates; a
-    HybridCache's states are updated in place.  Warm-up and capture do not move the cache forward:
+    HybridCache's states are updated in place.  ``kv_cache.adapter_slots`` may be written or replaced between steps (None: no
+    adapters), if the cache had some at the capture; another bank needs another capture.  Warm-up and capture do not move the cache forward:
     lengths and states are put back afterwards.
     """
 
@@ -589,6 +590,10 @@ class GraphedDecodeStep:
             self._prev = kv_cache.prev_embedding.clone()
             kv_cache.prev_embedding = self._prev
             in_place.append(self._prev)
+        # the adapters' slots are assigned to the cache as they come: the graph reads a copy, refreshed by every step, and this bank's weights
+        self._slots = self._bank = None
+        if getattr(kv_cache, "adapter_slots", None) is not None:
+            self._slots, self._bank = kv_cache.adapter_slots.clone(), model.adapters
         saved = [t.clone() for t in in_place]
         side = torch.cuda.Stream(dev)
         side.wait_stream(torch.cuda.current_stream(dev))
@@ -606,13 +611,33 @@ class GraphedDecodeStep:
     def _body(self):
         if self._prev is not None:
             self.cache.prev_embedding = self._prev
+        if self._slots is not None:
+            slots, self.cache.adapter_slots = self.cache.adapter_slots, self._slots
         logits = self.model.forward(self.ids, kv_cache=self.cache)[:, -1, :]
+        if self._slots is not None:
+            self.cache.adapter_slots = slots
         if self._prev is not None:
             self._prev.copy_(self.cache.prev_embedding)
             self.cache.prev_embedding = self._prev
         return logits
 
+    def _refresh_slots(self):
+        slots = getattr(self.cache, "adapter_slots", None)
+        if self._slots is None:
+            if slots is not None:
+                raise RuntimeError("the step was captured without adapters: capture another one")
+            return
+        if slots is None:
+            self._slots.fill_(-1)
+            return
+        if self.model.adapters is not self._bank:
+            raise RuntimeError("the step was captured with another bank of adapters: capture another one")
+        if slots.shape != self._slots.shape or slots.dtype != self._slots.dtype or slots.device != self._slots.device:
+            raise RuntimeError(f"adapter_slots must be {tuple(self._slots.shape)} {self._slots.dtype} on {self._slots.device}, as captured")
+        self._slots.copy_(slots)
+
     def step(self, ids):
+        self._refresh_slots()
         self.ids.copy_(ids, non_blocking=True)
         self.graph.replay()
         return self.logits
