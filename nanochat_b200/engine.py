@@ -571,7 +571,8 @@ class GraphedDecodeStep:
 
     ``step(ids)`` copies the token ids into the graph's input buffer, replays, and returns the
     logits buffer (B, vocab) — overwritten by the next call.  The smear state of a KVCache
-    (``kv_cache.prev_embedding``) is kept in a persistent buffer that the graph reads and updates; a
+    (``kv_cache.prev_embedding``) is kept in a persistent buffer that the graph reads and updates and that takes over what
+    the cache was given between two steps (a chunk's, a prompt's, None); a
     HybridCache's states are updated in place.  ``kv_cache.adapter_slots`` may be written or replaced between steps (None: no
     adapters), if the cache had some at the capture; another bank needs another capture.  Warm-up and capture do not move the cache forward:
     lengths and states are put back afterwards.
@@ -636,7 +637,18 @@ class GraphedDecodeStep:
             raise RuntimeError(f"adapter_slots must be {tuple(self._slots.shape)} {self._slots.dtype} on {self._slots.device}, as captured")
         self._slots.copy_(slots)
 
+    def _refresh_prev(self):
+        prev = getattr(self.cache, "prev_embedding", None)
+        if self._prev is None or prev is self._prev:
+            return
+        if prev is None:  # a smear of nothing
+            self._prev.zero_()
+        else:
+            self._prev.copy_(prev)
+        self.cache.prev_embedding = self._prev
+
     def step(self, ids):
+        self._refresh_prev()
         self._refresh_slots()
         self.ids.copy_(ids, non_blocking=True)
         self.graph.replay()

@@ -89,3 +89,35 @@ def test_a_captured_step_with_other_adapters(kind):
             torch.full((1024,), 1, dtype=torch.int32, device="cuda")  # what was freed is somebody else's
         got = step.step(ids[:, at:at + 1])
         assert torch.equal(got, m.forward(ids[:, at:at + 1], kv_cache=caches[1])[:, -1])
+
+
+def test_a_smear_state_that_was_replaced(no_cuda):
+    """By a chunk into the cache between two steps, by drafts that were taken back, by reset()."""
+    cache, model, ids, step = captured(None)
+    step.step(ids)
+    assert model.prev.eq(5).all()  # (the stand-in's replay writes nothing)
+    cache.prev_embedding = torch.full((2, 1, 4), 7.0)
+    step.step(ids)
+    assert model.prev.eq(7).all() and cache.prev_embedding is model.prev
+    cache.prev_embedding = None
+    step.step(ids)
+    assert model.prev.eq(0).all() and cache.prev_embedding is model.prev
+
+
+@pytest.mark.gpu
+def test_chunks_into_pages_between_captured_steps():
+    from nanochat_b200 import ops
+    from nanochat_b200.engine import PagedKVCache
+    from .test_chunks_behind_tokens import cache_of, make
+    m = make("cuda", torch.bfloat16, 256, 2, 1)
+    ids = torch.randint(0, 128, (2, 40), generator=torch.Generator().manual_seed(6)).cuda()
+    caches = [cache_of(PagedKVCache, m, 2, page_tokens=48) for _ in range(2)]
+    for cache in caches:
+        cache.reserve(48)
+        m.forward(ids[:, :8], kv_cache=cache)
+    step = GraphedDecodeStep(m, caches[0], ids[:, 8:9])
+    for lo, hi in ((8, 9), (9, 10), (10, 15), (15, 16), (16, 18), (18, 19), (19, 20)):
+        want = m.forward(ids[:, lo:hi], kv_cache=caches[1])[:, -1]
+        got = step.step(ids[:, lo:hi]) if hi == lo + 1 else m.forward(ids[:, lo:hi], kv_cache=caches[0])[:, -1]
+        assert torch.equal(got, want), (lo, hi)
+    assert ops.read_status("cuda") == 0
