@@ -60,7 +60,8 @@ def kv_attention(q, k, v, cos_sin_tables, window_size, kv_cache, layer_idx, new_
     and the 1.2 scale to q and k and appends k/v to the layer's cache; launch 2 attends.
     As in the reference the cache position is advanced once, after the last layer.
     Over a paged cache (whose pages the caller has reserved) ``new_tokens`` (int32 per row) says how many of a row's T slots
-    hold a token: the others leave the cache alone, their outputs are zero, and each row advances by its own count.
+    hold a token: the others leave the cache alone, their outputs are zero, and each row advances by its own count.  A count
+    outside 0..T sets a status bit and is taken as the nearest of them.
     Returns y of shape (B, T, Hq, D).
     """
     cos, sin = cos_sin_tables
@@ -86,7 +87,7 @@ def kv_attention(q, k, v, cos_sin_tables, window_size, kv_cache, layer_idx, new_
         else:
             y = ops.prefill_attention_paged(q2, k_cache, v_cache, kv_cache.block_table, seqlens, new_tokens, left)
         if layer_idx == kv_cache.n_layers - 1:
-            kv_cache.advance(T if new_tokens is None else new_tokens)
+            kv_cache.advance(T if new_tokens is None else new_tokens.clamp(0, T))  # as the launches take the counts
         return y
     if new_tokens is not None:
         raise NotImplementedError("counts of new tokens per row need a paged cache")
