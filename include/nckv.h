@@ -574,7 +574,7 @@ NCKV_API int nckv_gate_up(const void *h, const void *w, void *out, int rows, int
 /*
  * Low-rank adapters of B requests beside a projection that they share: row r of request b = r / T with s = slots[b] gets
  * out_r = bf16(y_r + scales[s] up_s (down_s x_r)), sums in fp32, or out_r = y_r where s < 0 (s >= S: the same, flagged).  bf16 y (B T, N),
- * x (B T, K) and out (B T, N) with row strides in elements (multiples of 8; out may be y), down (S, R, K) and up (S, N, R) packed; scales
+ * x (B T, K) and out (B T, N) with row strides in elements (multiples of 8; out may be y and shares no memory with x), down (S, R, K) and up (S, N, R) packed; scales
  * (S) fp32, slots (B) int32.  K, N and R are multiples of 8, R at most 128.  The workspace (16-byte aligned) is the call's own.
  */
 NCKV_API size_t nckv_adapters_workspace_bytes(int B, int T, int K, int N, int R, int S);

@@ -456,6 +456,16 @@ static int adapter_check_sizes(const char *name, int B, int T, int K, int N, int
     return NCKV_OK;
 }
 
+// Whether rows of `cols` elements `stride` apart lie on any of other ones.  At one distance rows may lie between each other (column slices of one
+// tensor); at two they have to be apart altogether.
+static bool adapter_rows_meet(const void *a, int64_t a_stride, int a_cols, const void *b, int64_t b_stride, int b_cols, long long rows) {
+    const long long lo_a = (long long)((uintptr_t)a / 2), lo_b = (long long)((uintptr_t)b / 2);
+    if (lo_a + (rows - 1) * a_stride + a_cols <= lo_b || lo_b + (rows - 1) * b_stride + b_cols <= lo_a) return false;
+    if (rows == 1 || a_stride != b_stride) return true;
+    const long long off = ((lo_b - lo_a) % a_stride + a_stride) % a_stride;
+    return off < a_cols || off + b_cols > a_stride;
+}
+
 }  // namespace nckv
 
 extern "C" size_t nckv_adapters_workspace_bytes(int B, int T, int K, int N, int R, int S) {
@@ -482,6 +492,15 @@ extern "C" int nckv_adapters(const void *y, int64_t y_stride, const void *x, int
     }
     if (((uintptr_t)y | (uintptr_t)x | (uintptr_t)down | (uintptr_t)up | (uintptr_t)out | (uintptr_t)workspace) & 15) {
         set_error("%s: tensors must be 16-byte aligned", name);
+        return NCKV_E_ARG;
+    }
+    const long long all = (long long)B * T;
+    if (adapter_rows_meet(out, out_stride, N, x, x_stride, K, all)) {
+        set_error("%s: the result and x share memory", name);
+        return NCKV_E_ARG;
+    }
+    if ((out != y || out_stride != y_stride) && adapter_rows_meet(out, out_stride, N, y, y_stride, N, all)) {
+        set_error("%s: the result is neither y nor beside it: they share memory", name);
         return NCKV_E_ARG;
     }
     if (workspace_bytes < nckv_adapters_workspace_bytes(B, T, K, N, R, S) || (workspace_bytes && !workspace)) {
