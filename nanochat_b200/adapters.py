@@ -11,6 +11,7 @@ A row whose slot is negative, and a cache without slots, run the projections alo
 import torch
 
 from . import ops
+from .gpt import gives_its_product_away
 
 PROJECTIONS = ("attn.c_q", "attn.c_k", "attn.c_v", "attn.c_proj", "mlp.c_fc", "mlp.c_proj")
 MAX_RANK = 128
@@ -83,10 +84,14 @@ class AdapterBank:
             self.scales[slot] = 0.0
 
     def at(self, layer, slots):
-        """What a layer does behind each of its products: ``add(name, y, x)`` -> y with the rows' adapters added in place."""
+        """What a layer does behind each of its products: ``add(name, y, x, module)`` -> y with the rows' adapters added, in place where
+        nobody else holds the product y of ``module`` (None: of no module)."""
         mine = self.layers[layer]
 
-        def add(name, y, x):
+        def add(name, y, x, module=None):
             pair = mine.get(name)
-            return y if pair is None else ops.add_adapters_(y, x, *pair, slots, self.scales)
+            if pair is None:
+                return y
+            op = ops.add_adapters_ if module is None or gives_its_product_away(module) else ops.add_adapters
+            return op(y, x, *pair, slots, self.scales)
         return add
