@@ -19,7 +19,7 @@ MAX_RANK = 128
 
 class AdapterBank:
     """``slots`` adapters of up to ``rank`` for the given projections of every layer of ``model`` (bfloat16, zero at
-    first); becomes ``model.adapters``."""
+    first); becomes ``model.adapters`` and goes to other devices with it."""
 
     def __init__(self, model, slots, rank, projections=PROJECTIONS):
         if slots <= 0 or not 0 < rank <= MAX_RANK:
@@ -82,6 +82,16 @@ class AdapterBank:
                     down[slot].zero_()
                     up[slot].zero_()
             self.scales[slot] = 0.0
+
+    def to(self, device):
+        """To the device that the model has gone to (of a bank without memory: empty slots)."""
+        def move(t):
+            return torch.zeros_like(t, device=device) if t.is_meta else t.to(device)
+        self.scales = move(self.scales)
+        for layer in self.layers:
+            for name, pair in layer.items():
+                layer[name] = tuple(move(t) for t in pair)
+        return self
 
     def at(self, layer, slots):
         """What a layer does behind each of its products: ``add(name, y, x, module)`` -> y with the rows' adapters added, in place where

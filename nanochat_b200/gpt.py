@@ -297,6 +297,12 @@ class GPT(nn.Module):
     def get_device(self):
         return self.transformer.wte.weight.device
 
+    def _apply(self, *args, **kwargs):
+        super()._apply(*args, **kwargs)
+        if self.adapters is not None:  # the adapters' weights have a type of their own
+            self.adapters.to(self.get_device())
+        return self
+
     def _resolve_dtype(self):
         if self.compute_dtype is None:
             self.compute_dtype = torch.bfloat16 if self.get_device().type == "cuda" else torch.float32

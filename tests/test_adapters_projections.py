@@ -96,3 +96,41 @@ def test_hooks_of_a_model_see_products_alone(T, fused):
     got = m.forward(ids, kv_cache=cache_of("dense", 2, [0, 1]))
     assert torch.equal(got, want)
     assert len(held) == 12 and all(torch.equal(a, b) for a, b in zip(held, copies))
+
+
+def test_a_bank_goes_where_its_model_goes():
+    m = GPT(GPTConfig(sequence_len=64, vocab_size=64, n_layer=2, n_head=2, n_kv_head=1, n_embd=256))
+    bank = AdapterBank(m, 2, 8, projections=("attn.c_q", "mlp.c_proj"))
+    down, up = torch.randn(8, 256), torch.randn(256, 8)
+    bank.load(1, {"transformer.h.1.attn.c_q.down": down, "transformer.h.1.attn.c_q.up": up}, scale=0.3)
+    before = bank.layers[1]["attn.c_q"][0]
+
+    def tensors():
+        return [bank.scales, *(t for layer in bank.layers for pair in layer.values() for t in pair)]
+    assert m.to(torch.bfloat16) is m and m.float() is m
+    assert bank.layers[1]["attn.c_q"][0] is before and bank.scales[1] == torch.tensor(0.3) and bank.scales.dtype == torch.float32  # only the model's type
+    m.to("meta")
+    assert len(tensors()) == 9 and all(t.is_meta and t.dtype == (torch.float32 if t is bank.scales else torch.bfloat16) for t in tensors())
+    m.to_empty(device="cpu")  # nothing is left of it: empty slots
+    assert all(t.device.type == "cpu" and not t.any() for t in tensors())
+    m.adapters = None
+    m.to("meta")
+    assert not bank.scales.is_meta
+
+
+@pytest.mark.gpu
+def test_a_model_made_on_the_host_runs_with_its_bank_on_the_gpu():
+    from .test_adapters_model_gpu import cache_of
+    torch.manual_seed(1)
+    m = GPT(GPTConfig(sequence_len=64, vocab_size=512, n_layer=3, n_head=4, n_kv_head=2, n_embd=512))
+    m.init_weights()
+    torch.nn.init.normal_(m.lm_head.weight, std=0.2)
+    torch.nn.init.normal_(m.transformer.h[0].mlp.c_proj.weight, std=0.05)
+    bank = AdapterBank(m, 2, 8)
+    bank.load(1, {"transformer.h.0.mlp.c_proj.down": torch.randn(4, 2048) * 2048 ** -0.5, "transformer.h.0.mlp.c_proj.up": torch.randn(512, 4)})
+    m.compute_dtype = torch.bfloat16
+    m = m.to(device="cuda", dtype=torch.bfloat16)
+    m.build_rotary()
+    ids = torch.arange(12, device="cuda")[None]
+    plain, got = (m.forward(ids, kv_cache=cache_of("dense", 1, slots)) for slots in (None, [1]))
+    assert not torch.equal(plain, got) and got.isfinite().all()
