@@ -361,6 +361,12 @@ class GPT(nn.Module):
         if self.cos.numel() == 0:
             self.build_rotary()
         assert T <= self.cos.size(1), f"Sequence length grew beyond the rotary embeddings cache: {T} > {self.cos.size(1)}"
+        slots = getattr(kv_cache, "adapter_slots", None)
+        if slots is not None and self.adapters is None:
+            raise ValueError("the cache's rows name adapters, the model has no bank of them")
+        if slots is not None and (slots.shape != (B,) or slots.dtype != torch.int32 or slots.device != idx.device or not slots.is_contiguous()):
+            raise ValueError(f"adapter_slots must be contiguous int32 on {idx.device} and name one slot for each of {B} rows, got {tuple(slots.shape)} "
+                             f"{slots.dtype} on {slots.device}")
         x = rms(self.transformer.wte(idx).to(dtype))
         if kv_cache is None:
             assert T > 1, "a forward pass without a KV cache needs T > 1"
@@ -384,11 +390,6 @@ class GPT(nn.Module):
         backout_at = self.config.n_layer // 2
         x_backout = None
         rope_tables = (self.cos, self.sin)
-        slots = getattr(kv_cache, "adapter_slots", None)
-        if slots is not None and self.adapters is None:
-            raise ValueError("the cache's rows name adapters, the model has no bank of them")
-        if slots is not None and slots.shape != (B,):
-            raise ValueError(f"adapter_slots must name one slot for each of {B} rows, got {tuple(slots.shape)}")
         if self.fused_glue and kv_cache is not None and x.is_cuda and x.dtype == torch.bfloat16 and \
                 (T == 1 or self._prompt_can_fuse(B, x.device)):
             return self._head(self._trunk_fused(idx, x, kv_cache, rope_tables, slots), logits_at)

@@ -121,3 +121,22 @@ def test_chunks_into_pages_between_captured_steps():
         got = step.step(ids[:, lo:hi]) if hi == lo + 1 else m.forward(ids[:, lo:hi], kv_cache=caches[0])[:, -1]
         assert torch.equal(got, want), (lo, hi)
     assert ops.read_status("cuda") == 0
+
+
+def test_a_pass_that_is_refused_leaves_the_cache_as_it_was():
+    from nanochat_b200.adapters import AdapterBank
+    from nanochat_b200.gpt import GPT, GPTConfig
+    m = GPT(GPTConfig(sequence_len=64, vocab_size=64, n_layer=1, n_head=2, n_kv_head=1, n_embd=256))
+    m.init_weights()
+    cache = KVCache(batch_size=2, num_heads=1, seq_len=8, head_dim=128, num_layers=1, device="cpu", dtype=torch.float32)
+    prev = cache.prev_embedding = torch.zeros(2, 1, 256)
+    cache.adapter_slots = ints(0, 0)
+    ids = torch.zeros(2, 1, dtype=torch.long)
+    with pytest.raises(ValueError, match="bank"):
+        m.forward(ids, kv_cache=cache)
+    m.adapters = AdapterBank(m, 1, 8)
+    for bad in (ints(0), ints(0, 0).long(), ints(0, 0).to("meta"), ints(0, 0, 0)[::2]):
+        cache.adapter_slots = bad
+        with pytest.raises(ValueError, match="adapter_slots"):
+            m.forward(ids, kv_cache=cache)
+    assert cache.prev_embedding is prev and cache.cache_seqlens.tolist() == [0, 0]
