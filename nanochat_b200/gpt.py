@@ -378,7 +378,7 @@ class GPT(nn.Module):
             if T <= 1:
                 before = prev
             elif prev is not None and getattr(kv_cache, "paged", False):  # a chunk behind tokens
-                before = torch.cat([prev.expand(B, -1, -1), x[:, :-1]], dim=1)
+                before = torch.cat([torch.where(kv_cache.cache_seqlens.view(B, 1, 1) > 0, prev, 0), x[:, :-1]], dim=1)
             else:  # the start of a sequence, and any chunk into dense rows, as gpt.py:438-449 has it
                 before = None
                 gate = self.smear_lambda.to(x.dtype) * torch.sigmoid(self.smear_gate(x[:, 1:, :24]))

@@ -70,6 +70,22 @@ def test_refused_drafts_are_taken_back():
     assert (got - want[:, 12:]).abs().max() <= 1e-4 * want.abs().max()
 
 
+def test_a_row_without_tokens_starts_a_sequence():
+    """Whatever the smear state still holds of what was there."""
+    m = make("cpu", torch.float32, 64, 2, 1)
+    ids = torch.randint(0, VOCAB, (2, 20), generator=torch.Generator().manual_seed(7))
+    with oracle_backend():
+        want = m.forward(ids)
+        cache = cache_of(Pages, m, 2)
+        m.forward(torch.cat([ids[:1].flip(1)[:, :8], ids[1:, :8]]), kv_cache=cache)
+        cache.cache_seqlens[0] = 0
+        cache.prev_embedding = cache.prev_embedding.clone()
+        cache.prev_embedding[0] = float("nan")
+        got = m.forward(torch.stack([ids[0, :12], ids[1, 8:]]), kv_cache=cache)
+    for a, b in ((got[0], want[0, :12]), (got[1], want[1, 8:])):
+        assert (a - b).abs().max() <= 1e-4 * want.abs().max()
+
+
 def test_dense_rows_do_what_the_reference_does():
     m = make("cpu", torch.float32, 64, 2, 1)
     ids = torch.randint(0, VOCAB, (1, 12), generator=torch.Generator().manual_seed(4))
