@@ -24,9 +24,11 @@
 // chunk_finish_kernel adds up partial sums in the order of the keys: results don't depend on timing.
 //
 // Bounds and figures.  Many new tokens: the tensor pipe and the softmax chain.  A key tile takes the pipe 640 cycles (S 8 products of 48 with both operands
-// in shared memory, O 4 of 64) and the exponentials 512; two CTAs of an SM get through one each in 1680, with the clock at 1.54 GHz under the power limit.
-// 2011 tokens behind 62 000 keys, 16 + 4 heads: 1094 us = 956 TFLOP/s; 8 prompts of 2048, 12 heads: 124 us = 829.  Few new tokens: the keys' bytes.
-// 2 x 8 tokens behind 49 000 keys, 12 heads: 88 us = 6.9 TB/s; 48 x 5 tokens behind 2048, 16 + 4 heads: 49 us = 4.2 TB/s, of which about 14 us are launches,
+// in shared memory, O 4 of 64) and the exponentials 512.  By the SMs' own counters the two CTAs of an SM get through one each in 1850 cycles, taken over a whole
+// pass of long rows (within a piece 1680), in 2500 where pieces have 17 (whole prompts of 2048: hand-over, masked tiles and tail besides).
+// 2011 tokens behind 62 000 keys, 16 + 4 heads: 1050 to 1100 us = 950 TFLOP/s, the clock at 1.42 GHz under the power limit; 8 prompts of 2048, 12 heads: 125 us =
+// 825 by themselves, 147 in a long run (1.50 GHz).  Few new tokens: the keys' bytes.  2 x 8 tokens, 12 heads, 457 MB of keys and values: 80 us = 5.7 TB/s, 562 MB:
+// 95 = 5.9; 48 x 5 tokens behind about 2048, 16 + 4 heads: 46 us for 210 MB, 52 for 229 = 4.4 to 4.5 TB/s, of which about 14 us are launches,
 // lengths, the first tiles' latency and the sums of parts, whatever the keys.  4 x 4 tokens of short rows: 7.5 us, launch and round trips.
 // Tried and slower: two threads per query row (147 us for the prompts), a warp of its own that cleans edge tiles (155), half or a quarter of the exponentials
 // as polynomials on the FMA pipe (131, 127), a maximum taken from the tile before, scores asked for before the stores of P are waited for (126).
