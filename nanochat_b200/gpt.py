@@ -299,7 +299,7 @@ class GPT(nn.Module):
 
     def _apply(self, *args, **kwargs):
         super()._apply(*args, **kwargs)
-        if self.adapters is not None:  # the adapters' weights have a type of their own
+        if getattr(self, "adapters", None) is not None:  # their weights have a type of their own
             self.adapters.to(self.get_device())
         return self
 
